@@ -41,7 +41,7 @@ DEFAULT_ROOT = os.path.join(os.path.dirname(os.path.dirname(os.path.dirname(os.p
 
 def install(reference_root: str = DEFAULT_ROOT) -> bool:
     """Returns True when every file is in place afterwards."""
-    if not os.path.isdir(reference_root):
+    if not all(os.path.isfile(os.path.join(reference_root, f)) for f in FILES):
         return all(os.path.exists(os.path.join(DEST, f)) for f in FILES)
     for rel in FILES:
         src = os.path.join(reference_root, rel)
