@@ -345,6 +345,77 @@ int b200_moe_grouped_gemm_nvfp4(int experts, const void* a_q, const void* sfa, i
 int b200_moe_combine(const void* y, int n, const int32_t* row_of, const float* topk_w, int tokens,
                      int top_k, int out_dtype, void* out, int64_t ldo, void* stream, int device);
 
+/* ---------------------------------------------------------------------------
+ * 8-bit floating-point matrices with a scale for each block of 128
+ *
+ * A matrix [rows, k] is e4m3 codes with row pitch ldq (a multiple of 16 bytes, at least k)
+ * and fp32 scales: one for each row and 128 columns, at sf[row * sf_row + (column / 128) *
+ * sf_col], or, for weights, one for each 128 x 128 block, at sf[(row / 128) * sf_row +
+ * (column / 128) * sf_col].  value = code * scale.  Any rows and k; the last block of a row
+ * may be shorter.  With a = max(|x|, 2^-100) over the block:
+ *   pow2 == 0   scale = a / 448, code = e4m3(448 x / a)
+ *   pow2 != 0   scale = the smallest power of two with a <= 448 scale, code = e4m3(x / scale)
+ * (round to nearest even).  A NaN keeps its place; an infinity makes the whole block NaN
+ * (pow2 == 0) or stays one (pow2 != 0).  The reference's experts take this format
+ * (moe/moe_fibench_ref.py:20-33).
+ * ------------------------------------------------------------------------- */
+int b200_fp8_quantize_rows(const void* x, int dtype, int rows, int k, int64_t ldx, void* q,
+                           int64_t ldq, float* sf, int64_t sf_row, int64_t sf_col, int pow2,
+                           void* stream, int device);
+int b200_fp8_quantize_blocks(const void* w, int dtype, int n, int k, int64_t ldw, void* q,
+                             int64_t ldq, float* sf, int64_t sf_row, int64_t sf_col, void* stream,
+                             int device);
+/* Values as fp16 or bf16 (exact for power-of-two scales whose values the type holds). */
+int b200_fp8_dequantize_rows(const void* q, int64_t ldq, const float* sf, int64_t sf_row,
+                             int64_t sf_col, int rows, int k, int out_dtype, void* out, int64_t ldo,
+                             void* stream, int device);
+
+/* b200_fp8_gemm: C [m, n] (fp16 or bf16, pitch ldc elements) = values(A) [m, k] . values(B)^T,
+ *   B [n, k] with 128 x 128 scales.  Products and sums inside a block of k are fp32 in tensor
+ *   memory, the sum over blocks is fp32, rounded once.  Any m, n, k > 0 with n % 8 == 0; row
+ *   pitches of A and B are multiples of 16, of C a multiple of 8. */
+int b200_fp8_gemm(const void* a, int64_t lda, const float* sfa, int64_t sfa_row, int64_t sfa_col,
+                  const void* b, int64_t ldb, const float* sfb, int64_t sfb_row, int64_t sfb_col,
+                  void* c, int64_t ldc, int out_dtype, int m, int n, int k, void* stream,
+                  int device, uint32_t* status);
+
+/* ---------------------------------------------------------------------------
+ * Gated feed-forward block in fp16 / bf16 (B200_DTYPE_*), forward and backward
+ *
+ *   g = x w1^T, u = x w2^T, h = act(g) * u         x [m, k], w1, w2 [n, k], h [m, n]
+ *   dg = dh * u * act'(g), du = dh * act(g)
+ *   dx = dg w1 + du w2, dw1 = dg^T x, dw2 = du^T x
+ *
+ * fp32 accumulation and gate, one rounding per result (h, dg, du, dx, dw).  Any m > 0; n and k
+ * multiples of 8; every pointer 16-byte aligned, row pitches (elements) multiples of 8, or of
+ * 16 for 8-bit matrices.  The unquantised, trainable sibling of b200_dual_gemm_nvfp4.
+ * ------------------------------------------------------------------------- */
+#define B200_ACT_SILU 0
+#define B200_ACT_GELU 1 /* tanh form */
+
+/* h; with qg != NULL also 8-bit copies of g and u (format above, pow2 scales, [m, n]) for
+ * b200_gated_grad_hidden_kept. */
+int b200_gated_forward(const void* x, int64_t ldx, const void* w1, int64_t ldw1, const void* w2,
+                       int64_t ldw2, int dtype, int act, void* h, int64_t ldh, void* qg, void* qu,
+                       int64_t ldq, float* sg, float* su, int64_t sf_row, int64_t sf_col, int m,
+                       int n, int k, void* stream, int device, uint32_t* status);
+/* dg and du, with g and u formed again from x and the weights. */
+int b200_gated_grad_hidden(const void* x, int64_t ldx, const void* w1, int64_t ldw1, const void* w2,
+                           int64_t ldw2, int dtype, int act, const void* dh, int64_t ld_dh, void* dg,
+                           void* du, int64_t ld_out, int m, int n, int k, void* stream, int device,
+                           uint32_t* status);
+/* dg and du, with the values of the 8-bit copies for g and u. */
+int b200_gated_grad_hidden_kept(const void* qg, const void* qu, int64_t ldq, const float* sg,
+                                const float* su, int64_t sf_row, int64_t sf_col, int dtype, int act,
+                                const void* dh, int64_t ld_dh, void* dg, void* du, int64_t ld_out,
+                                int m, int n, void* stream, int device);
+int b200_gated_grad_input(const void* dg, const void* du, int64_t ld_g, const void* w1, int64_t ldw1,
+                          const void* w2, int64_t ldw2, int dtype, void* dx, int64_t ld_dx, int m,
+                          int n, int k, void* stream, int device, uint32_t* status);
+int b200_gated_grad_weight(const void* dg, const void* du, int64_t ld_g, const void* x, int64_t ldx,
+                           int dtype, void* dw1, void* dw2, int64_t ld_dw, int m, int n, int k,
+                           void* stream, int device, uint32_t* status);
+
 /* Synchronise `stream`, copy the library-owned status word of `device` into
  * *out and clear it. */
 int b200_read_status(int device, void* stream, uint32_t* out);

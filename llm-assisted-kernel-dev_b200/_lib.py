@@ -20,6 +20,7 @@ E_NULL, E_SHAPE, E_ALIGN, E_WORKSPACE, E_VARIANT, E_DRIVER, E_LIMIT, E_CAPTURE =
 
 STATIC_MAX_GROUPS = 64
 DTYPE_F16, DTYPE_BF16 = 0, 1
+ACT_SILU, ACT_GELU = 0, 1
 
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
@@ -54,6 +55,17 @@ SIGNATURES = {
     "b200_moe_gemm_workspace_bytes": (_sz, [_i]),
     "b200_moe_grouped_gemm_nvfp4": (_i, [_i, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _i, _vp]),
     "b200_moe_combine": (_i, [_vp, _i, _vp, _vp, _i, _i, _i, _vp, _i64, _vp, _i]),
+    "b200_fp8_quantize_rows": (_i, [_vp, _i, _i, _i, _i64, _vp, _i64, _vp, _i64, _i64, _i, _vp, _i]),
+    "b200_fp8_quantize_blocks": (_i, [_vp, _i, _i, _i, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i]),
+    "b200_fp8_dequantize_rows": (_i, [_vp, _i64, _vp, _i64, _i64, _i, _i, _i, _vp, _i64, _vp, _i]),
+    "b200_fp8_gemm": (_i, [_vp, _i64, _vp, _i64, _i64] * 2 + [_vp, _i64] + [_i] * 4 + [_vp, _i, _vp]),
+    "b200_gated_forward": (_i, [_vp, _i64] * 3 + [_i, _i, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64] + [_i] * 3 +
+                           [_vp, _i, _vp]),
+    "b200_gated_grad_hidden": (_i, [_vp, _i64] * 3 + [_i, _i, _vp, _i64, _vp, _vp, _i64] + [_i] * 3 + [_vp, _i, _vp]),
+    "b200_gated_grad_hidden_kept": (_i, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _i, _i, _vp, _i64, _vp, _vp, _i64, _i, _i,
+                                         _vp, _i]),
+    "b200_gated_grad_input": (_i, [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _i, _vp, _i64] + [_i] * 3 + [_vp, _i, _vp]),
+    "b200_gated_grad_weight": (_i, [_vp, _vp, _i64, _vp, _i64, _i, _vp, _vp, _i64] + [_i] * 3 + [_vp, _i, _vp]),
     "b200_read_status": (_i, [_i, _vp, _u32p]),
     "b200_read_last_cycles": (_i, [_i, _vp, ctypes.POINTER(ctypes.c_uint64)]),
     "b200_probe_l2_feed": (_i, [_i, _i, _i, _i, _i, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double),

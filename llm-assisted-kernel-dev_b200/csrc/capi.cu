@@ -1402,3 +1402,5 @@ int b200_read_status(int device, void* stream, uint32_t* out) {
 }
 
 }  // extern "C"
+
+#include "capi_dense.cuh"

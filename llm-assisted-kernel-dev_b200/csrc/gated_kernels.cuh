@@ -1,0 +1,403 @@
+// Gated feed-forward block in 16-bit floating point, forward and backward, on CTA pairs (tcgen05 cta_group::2,
+// kind::f16, fp32 accumulators in tensor memory).
+//
+//   g = x W1^T, u = x W2^T, h = act(g) * u                              x [m, k], W1, W2 [n, k], h [m, n]
+//   dg = dh * u * act'(g), du = dh * act(g)
+//   dx = dg W1 + du W2,  dW1 = dg^T x,  dW2 = du^T x
+//
+// act(z) = z * sigma(c(z)): c(z) = z for SiLU, 2 sqrt(2/pi) (z + 0.044715 z^3) for the tanh form of GELU
+// (0.5 (1 + tanh t) = sigma(2t)), so both share act' = sigma + z sigma (1 - sigma) c'.
+//
+// One kernel template, four uses:
+//   Forward     256 x 128 tiles of g and u side by side (merged B: W1 rows in the first CTA, W2 rows in the
+//               second); the epilogue forms h and, on request, the 8-bit copies of g and u
+//   GradHidden  the same products again; the epilogue reads dh and writes dg and du
+//   GradInput   256 x 256 tiles of dx, k range = dg W1 then du W2 into the same accumulators; W as stored is
+//               MN-major for this product, which the MMA descriptor takes as it is: nothing is transposed
+//   GradWeight  256 x 256 tiles of dW1 and dW2 (two batches of one launch); both operands MN-major
+//
+// Bound by the tensor cores.  A 256 x 256 x 64 step of a pair takes 512 clocks of MMA at 4096 multiply-adds
+// per clock and SM; per SM it reads 32 KB by TMA (64 B/clk; this GPU feeds ~98) and 32 KB by MMA.
+// Six warps: 0-3 epilogue (each its 32 accumulator rows), 4 MMA issuer (first CTA), 5 TMA producer.
+#pragma once
+
+#include "dense_tiles.cuh"
+
+namespace b200 {
+
+enum class FfMode { Forward, GradHidden, GradInput, GradWeight };
+
+struct FfProblem {
+    CUtensorMap a[2], b[2];      // operands (see the modes above)
+    CUtensorMap out[2];          // h | dg, du | dx | dW1, dW2
+    CUtensorMap kept[2];         // 8-bit copies of g and u (Forward with keep)
+    const uint16_t* dh;          // GradHidden
+    long long ld_dh;
+    float* sf[2];                // scales of the 8-bit copies, [row * sf_row + block * sf_col]
+    long long sf_row, sf_col;
+    int rows, cols;              // of the outputs
+    int k_tiles, segments;       // 64-wide steps per segment; segments share the accumulators
+    int m_tiles, n_tiles, batches;
+    int gelu, keep;
+    uint32_t* status;
+};
+
+constexpr int kFfStages = 6;
+constexpr uint32_t kFfOperandBytes = 128u * 128u;            // 128 rows x 64 k (K-major) or 2 boxes of 64 x 64 (MN-major)
+constexpr uint32_t kFfStageBytes = 2u * kFfOperandBytes;
+constexpr uint32_t kFfStagingBytes = 4u * 8192u;             // per epilogue warp two boxes of 32 rows x 128 bytes
+constexpr int kFfThreads = 192;
+
+struct FfControl {
+    uint64_t full[kFfStages], empty[kFfStages];
+    uint64_t acc_full[2], acc_release[2], done;
+    uint32_t tmem_base, abort_flag;
+};
+constexpr uint32_t kFfSmemBytes = 1024u + kFfStages * kFfStageBytes + kFfStagingBytes + sizeof(FfControl);
+static_assert(kFfSmemBytes <= 227u * 1024u, "shared memory budget");
+
+// act(z) and, where asked for, act'(z).  sigma saturates to 0 and 1 without a NaN for finite z.
+struct GateValue { float value, slope; };
+template <bool kSlope> __device__ __forceinline__ GateValue gate(float z, int gelu) {
+    constexpr float kA = 1.5957691216057308f;    // 2 sqrt(2 / pi)
+    constexpr float kB = 0.044715f;
+    const float zz = z * z;
+    const float c = gelu ? kA * z * fmaf(kB, zz, 1.0f) : z;
+    const float s = __fdividef(1.0f, 1.0f + __expf(-c));
+    GateValue r;
+    r.value = z * s;
+    if constexpr (kSlope) {
+        const float dc = gelu ? kA * fmaf(3.0f * kB, zz, 1.0f) : 1.0f;
+        r.slope = fmaf(r.value * (1.0f - s), dc, s);
+    } else {
+        r.slope = 0.0f;
+    }
+    return r;
+}
+
+// h = act(g) u of 32 rows x 128 columns.
+template <bool kBf16>
+__device__ __forceinline__ void ff_epilogue_forward(const FfProblem& p, uint32_t acc, BoxWriter<2>& w, int row, int col) {
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+        const uint32_t box = w.acquire();
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+            uint32_t g[32], u[32];
+            tc_ld_x32(acc + half * 64 + c * 32, g);
+            tc_ld_x32(acc + 128 + half * 64 + c * 32, u);
+            tc_wait_ld();
+            float f[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = gate<false>(__uint_as_float(g[i]), p.gelu).value * __uint_as_float(u[i]);
+            put_chunk<kBf16>(w, box, c * 4, f);
+        }
+        w.send(box, &p.out[0], col + half * 64, row, row < p.rows && col + half * 64 < p.cols);
+    }
+}
+
+// 8-bit copy of one projection's 32 rows x 128 columns (a lane holds a whole block: its row's 128 columns).
+__device__ __forceinline__ void ff_epilogue_keep(const FfProblem& p, int which, uint32_t acc, BoxWriter<2>& w, int row, int col) {
+    float m = kAmaxFloor;
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        uint32_t v[32];
+        tc_ld_x32(acc + c * 32, v);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) m = fmaxf(m, fabsf(__uint_as_float(v[i])));
+    }
+    const PowerScale s(m);
+    const uint32_t box = w.acquire();
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        uint32_t v[32];
+        tc_ld_x32(acc + c * 32, v);
+        tc_wait_ld();
+        uint32_t q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            q[i] = pack_e4m3x4(s(__uint_as_float(v[4 * i])), s(__uint_as_float(v[4 * i + 1])),
+                               s(__uint_as_float(v[4 * i + 2])), s(__uint_as_float(v[4 * i + 3])));
+        w.put(box, 2 * c, q[0], q[1], q[2], q[3]);
+        w.put(box, 2 * c + 1, q[4], q[5], q[6], q[7]);
+    }
+    w.send(box, &p.kept[which], col, row, row < p.rows && col < p.cols);
+    const int r = row + w.lane;
+    if (r < p.rows && col < p.cols) p.sf[which][r * p.sf_row + (col / kFp8Block) * p.sf_col] = s.scale;
+}
+
+// dg and du of 32 rows x 128 columns from the accumulators and dh.
+template <bool kBf16>
+__device__ __forceinline__ void ff_epilogue_grad_hidden(const FfProblem& p, uint32_t acc, BoxWriter<2>& w, int row, int col) {
+    const int r = row + w.lane;
+    const uint16_t* dh = p.dh + r * p.ld_dh + col;
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+        const int c0 = half * 64;
+        // sixteen-byte pieces of this lane's dh row, 64 columns
+        uint4 d[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            d[j] = (r < p.rows && col + c0 + 8 * j < p.cols) ? *reinterpret_cast<const uint4*>(dh + c0 + 8 * j)
+                                                             : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            const uint32_t box = w.acquire();
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t g[32], u[32];
+                tc_ld_x32(acc + c0 + c * 32, g);
+                if (which == 0) tc_ld_x32(acc + 128 + c0 + c * 32, u);
+                tc_wait_ld();
+                float f[32];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float e[8];
+                    to_float8<kBf16>(d[c * 4 + j], e);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int at = 8 * j + i;
+                        if (which == 0)
+                            f[at] = e[i] * __uint_as_float(u[at]) * gate<true>(__uint_as_float(g[at]), p.gelu).slope;
+                        else
+                            f[at] = e[i] * gate<false>(__uint_as_float(g[at]), p.gelu).value;
+                    }
+                }
+                put_chunk<kBf16>(w, box, c * 4, f);
+            }
+            w.send(box, &p.out[which], col + c0, row, row < p.rows && col + c0 < p.cols);
+        }
+    }
+}
+
+// 32 rows x 256 columns of a plain product.
+template <bool kBf16>
+__device__ __forceinline__ void ff_epilogue_plain(const FfProblem& p, const CUtensorMap* map, uint32_t acc, BoxWriter<2>& w,
+                                                  int row, int col) {
+#pragma unroll 1
+    for (int part = 0; part < 4; ++part) {
+        const uint32_t box = w.acquire();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            uint32_t v[32];
+            tc_ld_x32(acc + part * 64 + c * 32, v);
+            tc_wait_ld();
+            float f[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
+            put_chunk<kBf16>(w, box, c * 4, f);
+        }
+        w.send(box, map, col + part * 64, row, row < p.rows && col + part * 64 < p.cols);
+    }
+}
+
+template <FfMode kMode, bool kBf16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfThreads, 1)
+ff_gemm_pair(const __grid_constant__ FfProblem p) {
+    constexpr bool kDual = kMode == FfMode::Forward || kMode == FfMode::GradHidden;
+    constexpr bool kAMn = kMode == FfMode::GradWeight;
+    constexpr bool kBMn = kMode == FfMode::GradWeight || kMode == FfMode::GradInput;
+    constexpr int kTileCols = kDual ? 128 : 256;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    FfControl* ctl = reinterpret_cast<FfControl*>(smem_raw + (smem_base - smem_u32(smem_raw)) + kFfStages * kFfStageBytes +
+                                                  kFfStagingBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_cta_rank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int tiles = p.m_tiles * p.n_tiles * p.batches;
+    const int steps = p.k_tiles * p.segments;
+    volatile uint32_t* abort_flag = &ctl->abort_flag;
+    griddep_launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kFfStages; ++s) {
+            mbar_init(smem_u32(&ctl->full[s]), 1);
+            mbar_init(smem_u32(&ctl->empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&ctl->acc_full[b]), 1);
+            mbar_init(smem_u32(&ctl->acc_release[b]), 8);    // four epilogue warps of each CTA; used in the first
+        }
+        mbar_init(smem_u32(&ctl->done), 1);
+        ctl->abort_flag = 0;
+        fence_mbar_init();
+        fence_proxy_async_smem();
+    }
+    if (warp == 4) {
+        tmem_alloc_pair(smem_u32(&ctl->tmem_base), 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    cluster_arrive();
+    cluster_wait();            // both CTAs' barriers exist
+    const uint32_t tmem_base = ctl->tmem_base;
+    griddep_wait();
+
+    if (warp == 5) {
+        // ------------------------------ producer: this CTA's rows of A and its half of B
+        uint32_t s = 0, ph = 0;
+        bool ok = true;
+        for (int tile = pair; ok && tile < tiles; tile += pairs) {
+            const TileAt t = banded_tile(tile, p.m_tiles, p.n_tiles);
+            const int a_row = t.m * 256 + static_cast<int>(rank) * 128;
+            const int b_row = kDual ? t.n * 128 : t.n * 256 + static_cast<int>(rank) * 128;
+            for (int i = 0; i < steps; ++i) {
+                const int seg = i >= p.k_tiles ? 1 : 0;
+                const int k0 = (i - seg * p.k_tiles) * 64;
+                if (!__all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->empty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense))) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t a_dst = smem_base + s * kFfStageBytes, b_dst = a_dst + kFfOperandBytes;
+                const uint32_t bar = map_to_cta(smem_u32(&ctl->full[s]), 0);
+                if (rank == 0) mbar_arrive_expect_tx_elect(smem_u32(&ctl->full[s]), 2 * kFfStageBytes);   // both CTAs' bytes
+                const CUtensorMap* ma = &p.a[kMode == FfMode::GradWeight ? t.batch : seg];
+                const CUtensorMap* mb = &p.b[kDual ? rank : (kMode == FfMode::GradInput ? seg : 0)];
+                if constexpr (kAMn) {
+                    tma_load_2d_pair_elect(a_dst, ma, bar, a_row, k0);
+                    tma_load_2d_pair_elect(a_dst + 8192, ma, bar, a_row + 64, k0);
+                } else {
+                    tma_load_2d_pair_elect(a_dst, ma, bar, k0, a_row);
+                }
+                if constexpr (kBMn) {
+                    tma_load_2d_pair_elect(b_dst, mb, bar, b_row, k0);
+                    tma_load_2d_pair_elect(b_dst + 8192, mb, bar, b_row + 64, k0);
+                } else {
+                    tma_load_2d_pair_elect(b_dst, mb, bar, k0, b_row);
+                }
+                if (++s == kFfStages) { s = 0; ph ^= 1u; }
+            }
+        }
+        if (!ok)
+            for (int i = 0; i < 64; ++i) __nanosleep(2000);   // error path: let copies in flight land
+        __syncwarp();
+    } else if (warp == 4) {
+        // ------------------------------ MMA issuer
+        if (rank == 0) {
+            constexpr uint32_t kIdesc = idesc_dense(256, 256, kBf16 ? 1u : 0u, kAMn, kBMn);
+            uint32_t s = 0, ph = 0;
+            int it = 0;
+            bool ok = true;
+            for (int tile = pair; ok && tile < tiles; tile += pairs, ++it) {
+                if (it >= 2)
+                    ok = __all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->acc_release[it & 1]), ((it >> 1) - 1) & 1, abort_flag,
+                                                           p.status, kStatusDense));
+                if (!ok) break;
+                tc_fence_after_sync();
+                const uint32_t acc = tmem_base + (it & 1) * 256;
+#pragma unroll 1
+                for (int i = 0; i < steps; ++i) {
+                    if (!__all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->full[s]), ph, abort_flag, p.status, kStatusDense))) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after_sync();
+                    const uint32_t a = dense_desc_lo<kAMn>(smem_base + s * kFfStageBytes);
+                    const uint32_t b = dense_desc_lo<kBMn>(smem_base + s * kFfStageBytes + kFfOperandBytes);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        tc_mma_f16_pair(acc, a + j * kDescStepK16<kAMn>, b + j * kDescStepK16<kBMn>, kIdesc, (i > 0 || j > 0) ? 1u : 0u);
+                    tc_commit_pair_both_elect(smem_u32(&ctl->empty[s]), 3);
+                    if (++s == kFfStages) { s = 0; ph ^= 1u; }
+                }
+                if (ok) tc_commit_pair_both_elect(smem_u32(&ctl->acc_full[it & 1]), 3);
+            }
+            tc_commit_pair_elect(smem_u32(&ctl->done));
+            mbar_wait<true>(smem_u32(&ctl->done), 0, abort_flag, p.status, kStatusDense);
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------ epilogue
+        BoxWriter<2> w{smem_base + kFfStages * kFfStageBytes + static_cast<uint32_t>(warp) * 8192u, lane, 0};
+        int it = 0;
+        for (int tile = pair; tile < tiles; tile += pairs, ++it) {
+            const TileAt t = banded_tile(tile, p.m_tiles, p.n_tiles);
+            if (!__all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->acc_full[it & 1]), (it >> 1) & 1, abort_flag, p.status, kStatusDense)))
+                break;
+            tc_fence_after_sync();
+            const uint32_t acc = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + (it & 1) * 256;
+            const int row = t.m * 256 + static_cast<int>(rank) * 128 + warp * 32, col = t.n * kTileCols;
+            if constexpr (kMode == FfMode::Forward) {
+                ff_epilogue_forward<kBf16>(p, acc, w, row, col);
+                if (p.keep) {
+                    ff_epilogue_keep(p, 0, acc, w, row, col);
+                    ff_epilogue_keep(p, 1, acc + 128, w, row, col);
+                }
+            } else if constexpr (kMode == FfMode::GradHidden) {
+                ff_epilogue_grad_hidden<kBf16>(p, acc, w, row, col);
+            } else {
+                ff_epilogue_plain<kBf16>(p, &p.out[t.batch], acc, w, row, col);
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&ctl->acc_release[it & 1]), 0));
+        }
+        if (lane == 0) bulk_wait_group_read_all();
+        __syncwarp();
+    }
+    // Nobody leaves while the partner may still signal its barriers or while MMAs run on this SM.
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    if (warp == 4) {
+        tc_fence_after_sync();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+// dg and du from the 8-bit copies of g and u: a streaming pass, 2 bytes of codes, 2 of dh and 4 of results per
+// element.  Eight columns per thread, kKeptUnits groups loaded before the first is used.
+constexpr int kKeptUnits = 2;
+template <bool kBf16>
+__global__ void __launch_bounds__(256)
+gated_grad_kept(const uint8_t* __restrict__ qg, const uint8_t* __restrict__ qu, long long ldq, const float* __restrict__ sg,
+                const float* __restrict__ su, long long sf_row, long long sf_col, const uint16_t* __restrict__ dh,
+                long long ld_dh, uint16_t* __restrict__ dg, uint16_t* __restrict__ du, long long ld_out, int rows, int n,
+                int gelu) {
+    griddep_launch_dependents();
+    griddep_wait();
+    const int per_row = n / 8;
+    const long long units = static_cast<long long>(rows) * per_row;
+    const long long first = static_cast<long long>(blockIdx.x) * (256 * kKeptUnits) + threadIdx.x;
+    uint2 a[kKeptUnits], b[kKeptUnits];
+    uint4 d[kKeptUnits];
+    float s1[kKeptUnits], s2[kKeptUnits];
+#pragma unroll
+    for (int i = 0; i < kKeptUnits; ++i) {
+        const long long u = first + i * 256;
+        if (u >= units) break;
+        const long long r = u / per_row;
+        const int col = static_cast<int>(u - r * per_row) * 8;
+        a[i] = *reinterpret_cast<const uint2*>(qg + r * ldq + col);
+        b[i] = *reinterpret_cast<const uint2*>(qu + r * ldq + col);
+        d[i] = *reinterpret_cast<const uint4*>(dh + r * ld_dh + col);
+        s1[i] = sg[r * sf_row + (col / kFp8Block) * sf_col];
+        s2[i] = su[r * sf_row + (col / kFp8Block) * sf_col];
+    }
+#pragma unroll
+    for (int i = 0; i < kKeptUnits; ++i) {
+        const long long u = first + i * 256;
+        if (u >= units) break;
+        const long long r = u / per_row;
+        const int col = static_cast<int>(u - r * per_row) * 8;
+        float e[8];
+        to_float8<kBf16>(d[i], e);
+        uint32_t og[4], ou[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 g = unpack_e4m3x2((j < 2 ? a[i].x : a[i].y) >> (16 * (j & 1)));
+            const float2 v = unpack_e4m3x2((j < 2 ? b[i].x : b[i].y) >> (16 * (j & 1)));
+            const GateValue g0 = gate<true>(g.x * s1[i], gelu), g1 = gate<true>(g.y * s1[i], gelu);
+            og[j] = pack_16<kBf16>(e[2 * j] * (v.x * s2[i]) * g0.slope, e[2 * j + 1] * (v.y * s2[i]) * g1.slope);
+            ou[j] = pack_16<kBf16>(e[2 * j] * g0.value, e[2 * j + 1] * g1.value);
+        }
+        *reinterpret_cast<uint4*>(dg + r * ld_out + col) = make_uint4(og[0], og[1], og[2], og[3]);
+        *reinterpret_cast<uint4*>(du + r * ld_out + col) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+    }
+}
+
+}  // namespace b200

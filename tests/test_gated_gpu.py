@@ -1,0 +1,311 @@
+"""Gated feed-forward block on the GPU, forward and backward, against a 64-bit implementation.
+
+Tolerances, with e = half a step of the type (bf16 2^-8, fp16 2^-11 relative) and S_y = the sum of magnitudes behind
+a sum y.  A projection of length k is ceil(k / 16) fp32 accumulations of 16 exact products, each off by at most 2^-22 of
+S (two bits below fp32's 24 for the alignment of the addends): d_g = ceil(k / 16) 2^-22 S_g.  act is 1.13-Lipschitz and its
+fp32 evaluation is good to 2^-18 of |act| (exp's argument carries |c| 2^-24, |c| < 40 where sigma is not negligible);
+act' is 1.7-Lipschitz, good to 2^-18.  So, to first order,
+    h    e |h| + |u| (1.13 d_g + 2^-18 |act|) + |act| d_u
+    dg   e |dg| + |dh| (|act'| d_u + |u| (1.7 d_g + 2^-18 (1 + |g|))),  du likewise
+    dx   e |dx| + the errors of dg and du carried through |w| + (2 n / 16 + 2) 2^-22 S_dx,  dw likewise."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16 = torch.bfloat16, torch.float16
+ALL = ("x", "w1", "w2")
+
+
+@pytest.fixture(scope="module")
+def dense():
+    from oracle import dense_oracle
+    return dense_oracle
+
+
+def _inputs(m, n, k, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed + m * 3 + n * 5 + k * 7)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    x, w1, w2 = r(m, k), r(n, k) * k ** -0.5, r(n, k) * k ** -0.5
+    return x.to(dtype), w1.to(dtype), w2.to(dtype), r(m, n).to(dtype)
+
+
+def _half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _floor(dtype):
+    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+
+
+def _within(got, want, tol, what):
+    assert got.shape == want.shape, what
+    d = (got.double() - want).abs()
+    assert not (d > tol).any(), (what, int((d > tol).sum()), d.max().item(), (d / tol).max().item())
+
+
+def _projections(x, w):
+    y = x.double() @ w.double().t()
+    return y, -(-x.shape[1] // 16) * 2.0 ** -22 * (x.double().abs() @ w.double().abs().t())
+
+
+def _forward_bound(dense, x, w1, w2, act):
+    g, dg = _projections(x, w1)
+    u, du = _projections(x, w2)
+    a, _ = dense.gate(g, act)
+    h = a * u
+    err = u.abs() * (1.13 * dg + 2.0 ** -18 * a.abs()) + (a.abs() + 1.13 * dg) * du
+    return h, err + _half_step(x.dtype) * (h.abs() + err) + _floor(x.dtype)
+
+
+def _hidden_bound(dense, g, d_g, u, d_u, dh, act, dtype):
+    a, da = dense.gate(g, act)
+    dh = dh.double()
+    dg, du = dh * u * da, dh * a
+    eg = dh.abs() * (da.abs() * d_u + (u.abs() + d_u) * (1.7 * d_g + 2.0 ** -18 * (1 + g.abs())))
+    eu = dh.abs() * (1.13 * d_g + 2.0 ** -18 * a.abs())
+    e = _half_step(dtype)
+    return dg, eg + e * (dg.abs() + eg) + _floor(dtype), du, eu + e * (du.abs() + eu) + _floor(dtype)
+
+
+def _grads_bound(dg, eg, du, eu, x, w1, w2, dtype):
+    x, w1, w2 = x.double(), w1.double(), w2.double()
+    m, n = dg.shape
+    e = _half_step(dtype)
+
+    def close(y, carried, total, steps):
+        t = carried + (steps + 2) * 2.0 ** -22 * total
+        return y, t + e * (y.abs() + t) + _floor(dtype)
+
+    dx = close(dg @ w1 + du @ w2, eg @ w1.abs() + eu @ w2.abs(), (dg.abs() + eg) @ w1.abs() + (du.abs() + eu) @ w2.abs(), n / 8)
+    dw1 = close(dg.t() @ x, eg.t() @ x.abs(), (dg.abs() + eg).t() @ x.abs(), m / 16)
+    dw2 = close(du.t() @ x, eu.t() @ x.abs(), (du.abs() + eu).t() @ x.abs(), m / 16)
+    return {"x": dx, "w1": dw1, "w2": dw2}
+
+
+SIZES = [(1, 8, 8), (1, 128, 256), (1, 1000, 2048), (2, 264, 72), (5, 136, 1000), (16, 512, 512), (33, 72, 136), (64, 1032, 264),
+         (100, 640, 1032), (128, 128, 64), (129, 136, 200), (256, 256, 128), (257, 392, 520), (300, 1024, 88), (520, 264, 776),
+         (1100, 520, 136)]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_forward(pkg, dense, m, n, k, dtype, act):
+    x, w1, w2, _ = _inputs(m, n, k, dtype)
+    got = pkg.gated.gated_ffn(x, w1, w2, activation=act)
+    _within(got, *_forward_bound(dense, x, w1, w2, act), "h")
+    assert torch.equal(got, pkg.gated.gated_ffn(x, w1, w2, activation=act))
+    assert pkg._lib.read_status(0) == 0
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_backward_from_the_inputs(pkg, dense, m, n, k, dtype, act):
+    x, w1, w2, dh = _inputs(m, n, k, dtype)
+    leaves = [t.requires_grad_() for t in (x, w1, w2)]
+    h = pkg.gated.gated_ffn(*leaves, activation=act)
+    grads = torch.autograd.grad(h, leaves, dh)
+    with torch.no_grad():
+        _within(h, *_forward_bound(dense, x, w1, w2, act), "h")
+        g, d_g = _projections(x, w1)
+        u, d_u = _projections(x, w2)
+        hidden = _hidden_bound(dense, g, d_g, u, d_u, dh, act, dtype)
+        want = _grads_bound(*hidden, x, w1, w2, dtype)
+        for name, got in zip(ALL, grads):
+            _within(got, *want[name], name)
+    assert pkg._lib.read_status(0) == 0
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_kept_copies_and_the_backward_pass_from_them(pkg, dense, m, n, k, dtype, act):
+    x, w1, w2, dh = _inputs(m, n, k, dtype)
+    leaves = [t.requires_grad_() for t in (x, w1, w2)]
+    h = pkg.gated.gated_ffn(*leaves, activation=act, keep="fp8")
+    w1s, w2s, qg, sg, qu, su, qx, sx = h.grad_fn.saved_tensors
+    assert torch.equal(h, pkg.gated.gated_ffn(x.detach(), w1.detach(), w2.detach(), activation=act))
+    grads = torch.autograd.grad(h, leaves, dh)
+    with torch.no_grad():
+        values = []
+        for q, s, w in ((qg, sg, w1), (qu, su, w2)):
+            y, d = _projections(x, w)
+            v = dense.row_values(q.float(), s)
+            steps = s.double().repeat_interleave(128, 1)[:, :n]
+            # half a step of e4m3 (2^-4 of the value, 2^-10 of the scale near zero), and the projection's own error
+            _within(v, y, 2.0 ** -4 * (y.abs() + d) + 2.0 ** -10 * steps + d, "kept values")
+            amax = torch.nn.functional.pad(y.abs() , (0, -n % 128)).view(m, -1, 128).amax(2)
+            slack = torch.nn.functional.pad(d, (0, -n % 128)).view(m, -1, 128).amax(2)
+            low, high = dense.pow2_scale((amax - slack).clamp_min(2.0 ** -100)), dense.pow2_scale((amax + slack).clamp_min(2.0 ** -100))
+            assert ((s.double() >= low) & (s.double() <= high)).all()
+            values.append(v)
+        codes, s = dense.quantize_rows(x, True)
+        assert torch.equal(qx.double(), codes) and torch.equal(sx.double(), s)
+        zero = torch.zeros_like(values[0])
+        hidden = _hidden_bound(dense, values[0], zero, values[1], zero, dh, act, dtype)
+        want = _grads_bound(*hidden, dense.row_values(qx.float(), sx), w1, w2, dtype)
+        for name, got in zip(ALL, grads):
+            _within(got, *want[name], name)
+    assert pkg._lib.read_status(0) == 0
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 16, 24), (130, 72, 264), (300, 520, 200)])
+def test_gradient_products_are_exact_on_small_integers(pkg, m, n, k):
+    """Integers whose products and sums stay below 2^8: bf16 holds every result, so any difference is a mistake."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    def ints(*s):
+        keep = torch.rand(s, generator=g, device="cuda") < 0.05
+        return (torch.randint(-2, 3, s, generator=g, device="cuda") * keep).to(BF16)
+    dg, du, x, w1, w2 = ints(m, n), ints(m, n), ints(m, k), ints(n, k), ints(n, k)
+    lib, st = pkg._lib.load(), torch.cuda.current_stream().cuda_stream
+    dx = torch.empty((m, k), dtype=BF16, device="cuda")
+    dw = torch.empty((2, n, k), dtype=BF16, device="cuda")
+    pkg._lib.check(lib.b200_gated_grad_input(dg.data_ptr(), du.data_ptr(), n, w1.data_ptr(), k, w2.data_ptr(), k, pkg._lib.DTYPE_BF16,
+                                             dx.data_ptr(), k, m, n, k, st, 0, None))
+    pkg._lib.check(lib.b200_gated_grad_weight(dg.data_ptr(), du.data_ptr(), n, x.data_ptr(), k, pkg._lib.DTYPE_BF16, dw[0].data_ptr(),
+                                              dw[1].data_ptr(), k, m, n, k, st, 0, None))
+    want = dg.double() @ w1.double() + du.double() @ w2.double()
+    assert want.abs().max() < 256 and torch.equal(dx.double(), want)
+    for got, d in zip(dw, (dg, du)):
+        want = d.double().t() @ x.double()
+        assert want.abs().max() < 256 and torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gradients_against_differences(pkg, dense, act):
+    """<dx, v> against (L(x + t v) - L(x - t v)) / 2t of the 64-bit forward: the quotient is off by t^2 / 6 times a
+    third derivative (t = 1e-4: below 1e-6 here), the gradient by its tolerance."""
+    m, n, k = 37, 136, 72
+    x, w1, w2, dh = _inputs(m, n, k, FP16)
+    leaves = [t.requires_grad_() for t in (x, w1, w2)]
+    grads = torch.autograd.grad(pkg.gated.gated_ffn(*leaves, activation=act), leaves, dh)
+    with torch.no_grad():
+        g, d_g = _projections(x, w1)
+        u, d_u = _projections(x, w2)
+        want = _grads_bound(*_hidden_bound(dense, g, d_g, u, d_u, dh, act, FP16), x, w1, w2, FP16)
+        at = [t.detach().double() for t in leaves]
+        for i, (name, got) in enumerate(zip(ALL, grads)):
+            v = torch.randn(at[i].shape, generator=torch.Generator(device="cuda").manual_seed(i), device="cuda").double()
+            def loss(t):
+                p = list(at)
+                p[i] = at[i] + t * v
+                return (dense.gated(*p, act) * dh.double()).sum()
+            quotient = (loss(1e-4) - loss(-1e-4)) / 2e-4
+            assert abs((got.double() * v).sum() - quotient) <= (want[name][1] * v.abs()).sum() + 1e-4 * quotient.abs() + 1e-4
+
+
+@pytest.mark.parametrize("keep", ["inputs", "fp8"])
+def test_only_what_is_asked_for(pkg, keep):
+    x, w1, w2, dh = _inputs(70, 136, 200, BF16)
+    full = [t.clone().requires_grad_() for t in (x, w1, w2)]
+    want = torch.autograd.grad(pkg.gated.gated_ffn(*full, keep=keep), full, dh)
+    for mask in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1), (0, 1, 1)):
+        leaves = [t.clone().requires_grad_(bool(f)) for t, f in zip((x, w1, w2), mask)]
+        got = torch.autograd.grad(pkg.gated.gated_ffn(*leaves, keep=keep), [t for t in leaves if t.requires_grad], dh)
+        for a, b in zip(got, [w for w, f in zip(want, mask) if f]):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("keep", ["inputs", "fp8"])
+def test_layouts_of_inputs_and_gradients(pkg, keep):
+    x, w1, w2, dh = _inputs(60, 136, 200, BF16)
+    leaves = [t.clone().requires_grad_() for t in (x, w1, w2)]
+    h = pkg.gated.gated_ffn(*leaves, keep=keep)
+    want = torch.autograd.grad(h, leaves, dh)
+    # leading dimensions; an input that is a slice of a wider buffer, one at an odd address, one transposed
+    wide = torch.zeros((60, 264), dtype=BF16, device="cuda")
+    wide[:, 8:208] = x
+    odd = torch.zeros(60 * 200 + 1, dtype=BF16, device="cuda")[1:].view(60, 200)
+    odd.copy_(x)
+    for xin in (x.view(3, 20, 200), wide[:, 8:208], odd, x.t().contiguous().t()):
+        xin = xin.detach().requires_grad_()
+        hh = pkg.gated.gated_ffn(xin, leaves[1], leaves[2], keep=keep)
+        assert hh.shape == (*xin.shape[:-1], 136) and torch.equal(hh.reshape(60, 136), h)
+        got = torch.autograd.grad(hh, (xin, leaves[1], leaves[2]), dh.view(hh.shape))
+        assert torch.equal(got[0].reshape(60, 200), want[0]) and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+    # a gradient that is one number seen through zero strides, and one that is transposed
+    ones = torch.autograd.grad(pkg.gated.gated_ffn(*leaves, keep=keep), leaves, torch.ones_like(h))
+    summed = torch.autograd.grad(pkg.gated.gated_ffn(*leaves, keep=keep).sum(), leaves)
+    turned = torch.autograd.grad(pkg.gated.gated_ffn(*leaves, keep=keep), leaves, dh.t().contiguous().t())
+    for a, b in list(zip(ones, summed)) + list(zip(turned, want)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("keep", ["inputs", "fp8"])
+def test_no_rows_and_rows_of_zeros(pkg, keep):
+    x, w1, w2, dh = _inputs(4, 136, 72, BF16)
+    leaves = [t.clone().requires_grad_() for t in (x[:0], w1, w2)]
+    h = pkg.gated.gated_ffn(*leaves, keep=keep)
+    dx, dw1, dw2 = torch.autograd.grad(h, leaves, dh[:0])
+    assert h.shape == (0, 136) and dx.shape == (0, 72) and not dw1.any() and not dw2.any()
+    # padded tokens: rows of zeros give zeros and add nothing to the weights' gradients
+    leaves = [t.clone().requires_grad_() for t in (x, w1, w2)]
+    padded = torch.zeros((300, 72), dtype=BF16, device="cuda")
+    padded[:4] = x
+    more = [padded.requires_grad_(), leaves[1], leaves[2]]
+    want = torch.autograd.grad(pkg.gated.gated_ffn(*leaves, keep=keep), leaves, dh)
+    dh_more = torch.ones((300, 136), dtype=BF16, device="cuda")
+    dh_more[:4] = dh
+    h = pkg.gated.gated_ffn(*more, keep=keep)
+    got = torch.autograd.grad(h, more, dh_more)
+    assert not h[4:].any() and torch.equal(got[0][:4], want[0])
+    assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+
+
+@pytest.mark.parametrize("keep", ["inputs", "fp8"])
+def test_training_step_on_a_side_stream_and_in_a_graph(pkg, keep):
+    x, w1, w2, dh = _inputs(130, 264, 200, BF16)
+    leaves = [t.requires_grad_() for t in (x, w1, w2)]
+
+    def step():
+        h = pkg.gated.gated_ffn(*leaves, keep=keep)
+        return (h.detach(), *torch.autograd.grad(h, leaves, dh))
+
+    want = [t.clone() for t in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for t in outs:
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    with torch.no_grad():
+        x.copy_(_inputs(130, 264, 200, BF16, seed=9)[0])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, step()))
+    del graph
+
+
+def test_kept_memory(pkg):
+    """keep="fp8" holds 2 n + k bytes per row and one scale for each 128 of them; keep="inputs" nothing new."""
+    m, n, k = 256, 1024, 512
+    x, w1, w2, _ = _inputs(m, n, k, BF16)
+    leaves = [t.requires_grad_() for t in (x, w1, w2)]
+    own = {t.data_ptr() for t in leaves}
+    size = lambda h: sum(t.numel() * t.element_size() for t in h.grad_fn.saved_tensors if t.data_ptr() not in own)  # noqa: E731
+    assert size(pkg.gated.gated_ffn(*leaves)) == 0
+    assert size(pkg.gated.gated_ffn(*leaves, keep="fp8")) == m * (2 * n + k) + 4 * m * (2 * n + k) // 128
+
+
+def test_block_then_quantised_projection(pkg, dense):
+    """The two operators in a row, as a serving layer runs them: gated block, then the fp8 down projection."""
+    x, w1, w2, _ = _inputs(150, 520, 264, BF16)
+    down, down_sf = pkg.fp8.quantize_fp8_weight(_inputs(1, 264, 520, BF16)[1])
+    y = pkg.fp8.fp8_linear(pkg.gated.gated_ffn(x, w1, w2), down, down_sf)
+    h = pkg.gated.gated_ffn(x, w1, w2)
+    codes, s = dense.quantize_rows(h, False)
+    av, bv = dense.row_values(codes, s), dense.block_values(down.float(), down_sf)
+    want, total = av @ bv.t(), av.abs() @ bv.abs().t()
+    tol = (4 * 2.0 ** -22 + (s.shape[1] + 2) * 2.0 ** -24) * total
+    _within(y, want, tol + _half_step(BF16) * (want.abs() + tol), "y")
