@@ -379,6 +379,17 @@ int b200_fp8_gemm(const void* a, int64_t lda, const float* sfa, int64_t sfa_row,
                   void* c, int64_t ldc, int out_dtype, int m, int n, int k, void* stream,
                   int device, uint32_t* status);
 
+/* b200_fp8_linear: y = values(quantised x) . values(w)^T in one call, x [m, k] fp16 or bf16 (row
+ *   pitch ldx, any alignment), y of the same type; equals b200_fp8_quantize_rows (pow2 = 0)
+ *   followed by b200_fp8_gemm bit for bit.  The weights start to load while x is quantised.
+ *   scratch: b200_fp8_linear_scratch_bytes(m, k) bytes, 16-byte aligned, free again once the call's
+ *   work on the stream is done. */
+size_t b200_fp8_linear_scratch_bytes(int m, int k);
+int b200_fp8_linear(const void* x, int64_t ldx, int dtype, const void* w, int64_t ldw,
+                    const float* sfw, int64_t sfw_row, int64_t sfw_col, void* y, int64_t ldy, int m,
+                    int n, int k, void* scratch, size_t scratch_bytes, void* stream, int device,
+                    uint32_t* status);
+
 /* ---------------------------------------------------------------------------
  * Gated feed-forward block in fp16 / bf16 (B200_DTYPE_*), forward and backward
  *

@@ -59,6 +59,8 @@ SIGNATURES = {
     "b200_fp8_quantize_blocks": (_i, [_vp, _i, _i, _i, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i]),
     "b200_fp8_dequantize_rows": (_i, [_vp, _i64, _vp, _i64, _i64, _i, _i, _i, _vp, _i64, _vp, _i]),
     "b200_fp8_gemm": (_i, [_vp, _i64, _vp, _i64, _i64] * 2 + [_vp, _i64] + [_i] * 4 + [_vp, _i, _vp]),
+    "b200_fp8_linear_scratch_bytes": (_sz, [_i, _i]),
+    "b200_fp8_linear": (_i, [_vp, _i64, _i, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i, _i, _i, _vp, _sz, _vp, _i, _vp]),
     "b200_gated_forward": (_i, [_vp, _i64] * 3 + [_i, _i, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64] + [_i] * 3 +
                            [_vp, _i, _vp]),
     "b200_gated_grad_hidden": (_i, [_vp, _i64] * 3 + [_i, _i, _vp, _i64, _vp, _vp, _i64] + [_i] * 3 + [_vp, _i, _vp]),

@@ -3,7 +3,7 @@
 #pragma once
 
 #include "fp8_gemm_kernels.cuh"
-#include "gated_kernels.cuh"
+#include "few_tokens_kernels.cuh"
 
 namespace b200 {
 namespace {
@@ -30,6 +30,18 @@ template <FfMode kMode> int opt_in_ff() {
     return rc ? rc : opt_in_smem(ff_gemm_pair<kMode, true>, kFfSmemBytes);
 }
 
+template <FewOp kOp, int kTokens> int opt_in_few() {
+    int rc = opt_in_smem(few_tokens_gemm<kOp, kTokens, false>, few_smem_bytes<kOp, kTokens>());
+    return rc ? rc : opt_in_smem(few_tokens_gemm<kOp, kTokens, true>, few_smem_bytes<kOp, kTokens>());
+}
+template <FewOp kOp> int opt_in_few_all() {
+    int rc;
+    if ((rc = opt_in_few<kOp, 16>())) return rc;
+    if ((rc = opt_in_few<kOp, 32>())) return rc;
+    if ((rc = opt_in_few<kOp, 64>())) return rc;
+    return opt_in_few<kOp, 128>();
+}
+
 // Lock, current device and per-device state of one call.
 struct DenseCall {
     std::lock_guard<std::mutex> lock;
@@ -47,6 +59,8 @@ struct DenseCall {
         if (ready) return;
         if ((rc = opt_in_smem(fp8_gemm_pair<false>, kFp8SmemBytes))) return;
         if ((rc = opt_in_smem(fp8_gemm_pair<true>, kFp8SmemBytes))) return;
+        if ((rc = opt_in_few_all<FewOp::Few8>())) return;
+        if ((rc = opt_in_few_all<FewOp::FewGated>())) return;
         if ((rc = opt_in_ff<FfMode::Forward>())) return;
         if ((rc = opt_in_ff<FfMode::GradHidden>())) return;
         if ((rc = opt_in_ff<FfMode::GradInput>())) return;
@@ -119,6 +133,51 @@ template <FfMode kMode> int launch_ff(const char* name, FfProblem& p, int dtype,
     return launch_dense(name, ff_gemm_pair<kMode, false>, dim3(grid), kFfThreads, kFfSmemBytes, call.stream, p);
 }
 
+// CTAs that share the k range of one tile: as many as the GPU has room for, with at least four steps each.
+int few_splits(long long tiles, int steps, int slots) {
+    int s = 8;
+    while (s > 1 && (tiles * s > slots || steps < 4 * s)) s >>= 1;
+    return s;
+}
+
+template <FewOp kOp, int kTokens, bool kBf16> int launch_few_as(FewProblem& p, DenseCall& call) {
+    using S = FewShape<kOp, kTokens>;
+    const int tiles = (p.n + 127) / 128, token_tiles = (p.m + kTokens - 1) / kTokens;
+    const int splits = few_splits(static_cast<long long>(tiles) * token_tiles, p.steps, call.st->sm_count * S::kCtasPerSm);
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof cfg);
+    cfg.gridDim = dim3(tiles * splits, token_tiles, 1);
+    cfg.blockDim = dim3(kFewThreads, 1, 1);
+    cfg.dynamicSmemBytes = few_smem_bytes<kOp, kTokens>();
+    cfg.stream = call.stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    B200_CUDA(cudaLaunchKernelEx(&cfg, few_tokens_gemm<kOp, kTokens, kBf16>, p));
+    ++g_launches;
+    g_last_kernel = kOp == FewOp::Few8 ? "few_tokens_gemm<Few8>" : "few_tokens_gemm<FewGated>";
+    return 0;
+}
+// The token tile: the smallest that holds all tokens, up to 128.
+int few_tokens_tile(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128; }
+template <FewOp kOp> int launch_few(FewProblem& p, int dtype, DenseCall& call, uint32_t* status) {
+    p.status = status ? status : call.st->status;
+    const bool bf16 = dtype == B200_DTYPE_BF16;
+    switch (few_tokens_tile(p.m)) {
+        case 16: return bf16 ? launch_few_as<kOp, 16, true>(p, call) : launch_few_as<kOp, 16, false>(p, call);
+        case 32: return bf16 ? launch_few_as<kOp, 32, true>(p, call) : launch_few_as<kOp, 32, false>(p, call);
+        case 64: return bf16 ? launch_few_as<kOp, 64, true>(p, call) : launch_few_as<kOp, 64, false>(p, call);
+        default: return bf16 ? launch_few_as<kOp, 128, true>(p, call) : launch_few_as<kOp, 128, false>(p, call);
+    }
+}
+constexpr int kFewMost = 256;
+
 // Maps and sizes that the forward pass and its recomputation share.
 int ff_projections(FfProblem& p, const void* x, long long ldx, const void* w1, long long ldw1, const void* w2, long long ldw2,
                    int act, int m, int n, int k) {
@@ -135,6 +194,82 @@ int ff_projections(FfProblem& p, const void* x, long long ldx, const void* w1, l
     p.batches = 1;
     p.gelu = act == B200_ACT_GELU;
     return 0;
+}
+
+int quantize_rows_launch(const char* what, const void* x, int dtype, int rows, int k, long long ldx, void* q, long long ldq,
+                         float* sf, long long sf_row, long long sf_col, int pow2, DenseCall& call) {
+    const long long units = static_cast<long long>(rows) * ((k + kFp8Block - 1) / kFp8Block);
+    constexpr int kPerBlock = kRowThreads / 16 * kRowUnits;
+    const long long blocks = (units + kPerBlock - 1) / kPerBlock;
+    if (blocks > 0x7FFFFFFFll) return fail(B200_E_LIMIT, "%s: %d rows and k=%d are too many blocks for one launch", what, rows, k);
+    const bool vec = aligned16(x) && ldx % 8 == 0;
+    const uint16_t* src = static_cast<const uint16_t*>(x);
+    uint8_t* qp = static_cast<uint8_t*>(q);
+    auto go = [&](auto* kernel) {
+        return launch_dense("fp8_quantize_rows", kernel, dim3(static_cast<unsigned>(blocks)), kRowThreads, 0u, call.stream, src, ldx,
+                            rows, k, qp, ldq, sf, sf_row, sf_col);
+    };
+    if (dtype == B200_DTYPE_BF16) {
+        if (pow2) return vec ? go(&fp8_quantize_rows<true, true, true>) : go(&fp8_quantize_rows<true, true, false>);
+        return vec ? go(&fp8_quantize_rows<true, false, true>) : go(&fp8_quantize_rows<true, false, false>);
+    }
+    if (pow2) return vec ? go(&fp8_quantize_rows<false, true, true>) : go(&fp8_quantize_rows<false, true, false>);
+    return vec ? go(&fp8_quantize_rows<false, false, true>) : go(&fp8_quantize_rows<false, false, false>);
+}
+
+// One quantised operand: codes, row pitch, scales and their strides.
+struct Fp8Matrix {
+    const void* q;
+    long long ld;
+    const float* sf;
+    long long sf_row, sf_col;
+};
+// Codes of [m, k] in the linear layer's scratch, the scales behind them.
+size_t fp8_codes_bytes(int m, int k) { return static_cast<size_t>(m) * ((k + 15) / 16 * 16); }
+
+// `after_quantiser`: the launch before this one on the stream is fp8_quantize_rows, which has waited for all before it
+// by the time this kernel starts and does not write the weights.
+int fp8_gemm_launch(const Fp8Matrix& a, const Fp8Matrix& b, void* c, long long ldc, int out_dtype, int m, int n, int k,
+                    bool after_quantiser, DenseCall& call, uint32_t* status) {
+    int rc;
+    if (m <= kFewMost) {
+        FewProblem p;
+        memset(&p, 0, sizeof p);
+        if ((rc = encode_matrix_map(&p.w[0], b.q, 1, k, n, b.ld, 128, 128))) return rc;
+        if ((rc = encode_matrix_map(&p.x, a.q, 1, k, m, a.ld, 128, few_tokens_tile(m)))) return rc;
+        p.sfa = a.sf;
+        p.sfa_row = a.sf_row;
+        p.sfa_col = a.sf_col;
+        p.sfb = b.sf;
+        p.sfb_row = b.sf_row;
+        p.sfb_col = b.sf_col;
+        p.c = static_cast<uint16_t*>(c);
+        p.ldc = ldc;
+        p.m = m;
+        p.n = n;
+        p.steps = (k + kFp8Block - 1) / kFp8Block;
+        p.weights_early = after_quantiser;
+        return launch_few<FewOp::Few8>(p, out_dtype, call, status);
+    }
+    Fp8Problem p;
+    if ((rc = encode_matrix_map(&p.a, a.q, 1, k, m, a.ld, 128, 128))) return rc;
+    if ((rc = encode_matrix_map(&p.b, b.q, 1, k, n, b.ld, 128, 128))) return rc;
+    if ((rc = encode_matrix_map(&p.c, c, 2, n, m, ldc, 64, 32))) return rc;
+    p.sfa = a.sf;
+    p.sfa_row = a.sf_row;
+    p.sfa_col = a.sf_col;
+    p.sfb = b.sf;
+    p.sfb_row = b.sf_row;
+    p.sfb_col = b.sf_col;
+    p.m = m;
+    p.n = n;
+    p.k_tiles = (k + kFp8Block - 1) / kFp8Block;
+    p.m_tiles = (m + 255) / 256;
+    p.n_tiles = (n + 255) / 256;
+    p.status = status ? status : call.st->status;
+    const int grid = pair_grid(static_cast<long long>(p.m_tiles) * p.n_tiles, call.st->sm_count);
+    auto* kernel = out_dtype == B200_DTYPE_BF16 ? &fp8_gemm_pair<true> : &fp8_gemm_pair<false>;
+    return launch_dense("fp8_gemm_pair", kernel, dim3(grid), kFp8Threads, kFp8SmemBytes, call.stream, p);
 }
 
 }  // namespace
@@ -155,25 +290,7 @@ int b200_fp8_quantize_rows(const void* x, int dtype, int rows, int k, int64_t ld
     if ((rc = check_matrix(what, "q", q, ldq, k, 1))) return rc;
     DenseCall call(device, stream);
     if (call.rc) return call.rc;
-    const long long units = static_cast<long long>(rows) * ((k + kFp8Block - 1) / kFp8Block);
-    constexpr int kPerBlock = kRowThreads / 16 * kRowUnits;
-    const long long blocks = (units + kPerBlock - 1) / kPerBlock;
-    if (blocks > 0x7FFFFFFFll) return fail(B200_E_LIMIT, "%s: rows=%d and k=%d are too many blocks for one launch", what, rows, k);
-    const bool vec = aligned16(x) && ldx % 8 == 0;
-    const uint16_t* src = static_cast<const uint16_t*>(x);
-    uint8_t* qp = static_cast<uint8_t*>(q);
-#define B200_ROWS(bf, p2, v)                                                                                                  \
-    return launch_dense("fp8_quantize_rows", fp8_quantize_rows<bf, p2, v>, dim3(static_cast<unsigned>(blocks)), kRowThreads, \
-                        0u, call.stream, src, static_cast<long long>(ldx), rows, k, qp, static_cast<long long>(ldq), sf,     \
-                        static_cast<long long>(sf_row), static_cast<long long>(sf_col))
-    if (dtype == B200_DTYPE_BF16) {
-        if (pow2) { if (vec) B200_ROWS(true, true, true); else B200_ROWS(true, true, false); }
-        else { if (vec) B200_ROWS(true, false, true); else B200_ROWS(true, false, false); }
-    } else {
-        if (pow2) { if (vec) B200_ROWS(false, true, true); else B200_ROWS(false, true, false); }
-        else { if (vec) B200_ROWS(false, false, true); else B200_ROWS(false, false, false); }
-    }
-#undef B200_ROWS
+    return quantize_rows_launch(what, x, dtype, rows, k, ldx, q, ldq, sf, sf_row, sf_col, pow2, call);
 }
 
 int b200_fp8_quantize_blocks(const void* w, int dtype, int n, int k, int64_t ldw, void* q, int64_t ldq, float* sf,
@@ -234,25 +351,37 @@ int b200_fp8_gemm(const void* a, int64_t lda, const float* sfa, int64_t sfa_row,
     if ((rc = check_matrix(what, "c", c, ldc, n, 2))) return rc;
     DenseCall call(device, stream);
     if (call.rc) return call.rc;
-    Fp8Problem p;
-    if ((rc = encode_matrix_map(&p.a, a, 1, k, m, lda, 128, 128))) return rc;
-    if ((rc = encode_matrix_map(&p.b, b, 1, k, n, ldb, 128, 128))) return rc;
-    if ((rc = encode_matrix_map(&p.c, c, 2, n, m, ldc, 64, 32))) return rc;
-    p.sfa = sfa;
-    p.sfa_row = sfa_row;
-    p.sfa_col = sfa_col;
-    p.sfb = sfb;
-    p.sfb_row = sfb_row;
-    p.sfb_col = sfb_col;
-    p.m = m;
-    p.n = n;
-    p.k_tiles = (k + kFp8Block - 1) / kFp8Block;
-    p.m_tiles = (m + 255) / 256;
-    p.n_tiles = (n + 255) / 256;
-    p.status = status ? status : call.st->status;
-    const int grid = pair_grid(static_cast<long long>(p.m_tiles) * p.n_tiles, call.st->sm_count);
-    auto* kernel = out_dtype == B200_DTYPE_BF16 ? &fp8_gemm_pair<true> : &fp8_gemm_pair<false>;
-    return launch_dense("fp8_gemm_pair", kernel, dim3(grid), kFp8Threads, kFp8SmemBytes, call.stream, p);
+    const Fp8Matrix ma{a, lda, sfa, sfa_row, sfa_col}, mb{b, ldb, sfb, sfb_row, sfb_col};
+    return fp8_gemm_launch(ma, mb, c, ldc, out_dtype, m, n, k, false, call, status);
+}
+
+size_t b200_fp8_linear_scratch_bytes(int m, int k) {
+    if (m <= 0 || k <= 0) return 0;
+    return fp8_codes_bytes(m, k) + static_cast<size_t>(m) * ((k + kFp8Block - 1) / kFp8Block) * 4;
+}
+
+int b200_fp8_linear(const void* x, int64_t ldx, int dtype, const void* w, int64_t ldw, const float* sfw, int64_t sfw_row,
+                    int64_t sfw_col, void* y, int64_t ldy, int m, int n, int k, void* scratch, size_t scratch_bytes,
+                    void* stream, int device, uint32_t* status) {
+    const char* what = "fp8 linear";
+    int rc;
+    if (!x || !sfw) return fail(B200_E_NULL, "%s: NULL tensor pointer", what);
+    if ((rc = check_dtype(what, dtype))) return rc;
+    if ((rc = check_positive(what, m, n, k))) return rc;
+    if (n % 8) return fail(B200_E_SHAPE, "%s: n=%d is not a multiple of 8", what, n);
+    if (ldx < k) return fail(B200_E_ALIGN, "%s: ldx=%lld must be at least k=%d", what, (long long)ldx, k);
+    if ((rc = check_matrix(what, "w", w, ldw, k, 1))) return rc;
+    if ((rc = check_matrix(what, "y", y, ldy, n, 2))) return rc;
+    if (!scratch || !aligned16(scratch) || scratch_bytes < b200_fp8_linear_scratch_bytes(m, k))
+        return fail(B200_E_WORKSPACE, "%s: needs %zu scratch bytes, 16-byte aligned", what, b200_fp8_linear_scratch_bytes(m, k));
+    DenseCall call(device, stream);
+    if (call.rc) return call.rc;
+    uint8_t* q = static_cast<uint8_t*>(scratch);
+    float* sf = reinterpret_cast<float*>(q + fp8_codes_bytes(m, k));
+    const int64_t ldq = (k + 15) / 16 * 16;
+    if ((rc = quantize_rows_launch(what, x, dtype, m, k, ldx, q, ldq, sf, 1, m, 0, call))) return rc;
+    const Fp8Matrix ma{q, ldq, sf, 1, m}, mb{w, ldw, sfw, sfw_row, sfw_col};
+    return fp8_gemm_launch(ma, mb, y, ldy, dtype, m, n, k, true, call, status);
 }
 
 int b200_gated_forward(const void* x, int64_t ldx, const void* w1, int64_t ldw1, const void* w2, int64_t ldw2, int dtype, int act,
@@ -273,6 +402,20 @@ int b200_gated_forward(const void* x, int64_t ldx, const void* w1, int64_t ldw1,
     }
     DenseCall call(device, stream);
     if (call.rc) return call.rc;
+    if (m <= kFewMost && !keep) {
+        FewProblem f;
+        memset(&f, 0, sizeof f);
+        if ((rc = encode_matrix_map(&f.w[0], w1, 2, k, n, ldw1, 64, 128))) return rc;
+        if ((rc = encode_matrix_map(&f.w[1], w2, 2, k, n, ldw2, 64, 128))) return rc;
+        if ((rc = encode_matrix_map(&f.x, x, 2, k, m, ldx, 64, few_tokens_tile(m)))) return rc;
+        f.c = static_cast<uint16_t*>(h);
+        f.ldc = ldh;
+        f.m = m;
+        f.n = n;
+        f.steps = (k + 63) / 64;
+        f.gelu = act == B200_ACT_GELU;
+        return launch_few<FewOp::FewGated>(f, dtype, call, status);
+    }
     FfProblem p;
     memset(&p, 0, sizeof p);
     if ((rc = ff_projections(p, x, ldx, w1, ldw1, w2, ldw2, act, m, n, k))) return rc;

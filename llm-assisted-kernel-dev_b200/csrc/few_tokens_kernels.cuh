@@ -1,0 +1,332 @@
+// The fp8 linear layer and the gated block's forward pass for few tokens (a decoding step, a short prompt).
+//
+// With m of a few dozen rows these products read each weight once and do little with it: the floor is the weight's
+// bytes at memory bandwidth, and 256-row tiles would leave most SMs idle (n / 256 tiles).  So the operands change
+// places - C^T = W A^T: 128 rows of W are the MMA's M, 16 to 128 tokens its N - and the k range of a tile is cut
+// over a cluster of up to eight CTAs, so that every SM streams weights.  The partial sums meet through distributed
+// shared memory, added in rank order: no workspace, no atomics, the same bits on every run.
+//
+//   Few8      fp8: fp32 sums of one 128-wide block in tensor memory, scaled and added up in registers (one weight
+//             row per lane, one column per token), as in fp8_gemm_pair
+//   FewGated  16-bit: g and u of the same rows and tokens side by side in tensor memory, h formed after the exchange
+//
+// Seven warps: 0-3 sums and results, 4 MMA issuer, 5 weight loads, 6 token loads (and their scales).
+#pragma once
+
+#include "dense_tiles.cuh"
+#include "gated_kernels.cuh"
+
+namespace b200 {
+
+enum class FewOp { Few8, FewGated };
+
+struct FewProblem {
+    CUtensorMap w[2], x;
+    const float* sfa;            // Few8: token scales, [token * sfa_row + block * sfa_col]
+    const float* sfb;            // Few8: weight scales, [(row / 128) * sfb_row + block * sfb_col]
+    long long sfa_row, sfa_col, sfb_row, sfb_col;
+    uint16_t* c;
+    long long ldc;
+    int m, n, steps;             // steps: 128-byte pieces of k (128 e4m3, 64 16-bit)
+    int gelu;
+    int weights_early;           // the kernel before this one on the stream is known not to write the weights and to have waited
+                                 // for all before it: weight loads need not wait for it
+    uint32_t* status;
+};
+
+template <FewOp kOp, int kTokens> struct FewShape {
+    static constexpr bool kFp8 = kOp == FewOp::Few8;
+    static constexpr uint32_t kWeightBytes = (kFp8 ? 1u : 2u) * 16384u;     // 128 rows x 128 bytes of each weight
+    static constexpr uint32_t kTokenBytes = kTokens * 128u;
+    static constexpr uint32_t kStageBytes = kWeightBytes + kTokenBytes;
+    // two CTAs on an SM up to 64 (fp8) or 32 tokens, one beyond: registers and stages
+    static constexpr int kCtasPerSm = kTokens <= (kFp8 ? 64 : 32) ? 2 : 1;
+    static constexpr int kStages = static_cast<int>((kCtasPerSm == 2 ? 108u * 1024u : 200u * 1024u) / kStageBytes);
+    static constexpr uint32_t kTmemCols = 2 * kTokens;                      // two block buffers, or g and u
+    // partial sums for the exchange take the place of the stages
+    static_assert((kFp8 ? 1u : 2u) * kTokens * 512u <= kStages * kStageBytes, "exchange area");
+    static_assert(kStageBytes % 1024 == 0, "stages keep the alignment of the swizzle");
+};
+template <FewOp kOp, int kTokens> struct FewControl {
+    using S = FewShape<kOp, kTokens>;
+    uint64_t wfull[S::kStages], tfull[S::kStages], empty[S::kStages];
+    uint64_t sfull[S::kStages], sempty[S::kStages];
+    uint64_t acc_full[2], acc_release[2];
+    uint32_t tmem_base, abort_flag;
+    alignas(16) float scale[S::kStages][kTokens];
+};
+template <FewOp kOp, int kTokens> constexpr uint32_t few_smem_bytes() {
+    using S = FewShape<kOp, kTokens>;
+    return 1024u + S::kStages * S::kStageBytes + sizeof(FewControl<kOp, kTokens>);
+}
+constexpr int kFewThreads = 224;
+
+// 4-byte asynchronous copy (zero when not valid) and an arrival when this thread's copies so far have landed.
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool valid) {
+    const int bytes = valid ? 4 : 0;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive_noinc(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_shared_f32(uint32_t addr, float v) {
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+template <bool kBf16> __device__ __forceinline__ uint16_t to_16(float v) { return static_cast<uint16_t>(pack_16<kBf16>(v, 0.0f)); }
+
+template <int kN> __device__ __forceinline__ void tc_ld_cols(uint32_t taddr, uint32_t (&v)[kN]) {
+    static_assert(kN == 16 || kN == 32, "columns per load");
+    if constexpr (kN == 16) tc_ld_x16(taddr, v);
+    else tc_ld_x32(taddr, v);
+}
+
+template <FewOp kOp, int kTokens, bool kBf16>
+__global__ void __launch_bounds__(kFewThreads, FewShape<kOp, kTokens>::kCtasPerSm)
+few_tokens_gemm(const __grid_constant__ FewProblem p) {
+    using S = FewShape<kOp, kTokens>;
+    constexpr bool kFp8 = S::kFp8;
+    constexpr int kStages = S::kStages;
+    constexpr int kChunk = kTokens < 32 ? kTokens : 32;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    auto* ctl = reinterpret_cast<FewControl<kOp, kTokens>*>(smem_raw + (smem_base - smem_u32(smem_raw)) + kStages * S::kStageBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t splits;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
+    const uint32_t rank = cluster_cta_rank();
+    const int w_row = static_cast<int>(blockIdx.x / splits) * 128;
+    const int token0 = blockIdx.y * kTokens;
+    const int begin = static_cast<int>(static_cast<long long>(p.steps) * rank / splits);
+    const int count = static_cast<int>(static_cast<long long>(p.steps) * (rank + 1) / splits) - begin;
+    volatile uint32_t* abort_flag = &ctl->abort_flag;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(smem_u32(&ctl->wfull[s]), 1);
+            mbar_init(smem_u32(&ctl->tfull[s]), 1);
+            mbar_init(smem_u32(&ctl->empty[s]), 1);
+            mbar_init(smem_u32(&ctl->sfull[s]), 32);
+            mbar_init(smem_u32(&ctl->sempty[s]), 4);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&ctl->acc_full[b]), 1);
+            mbar_init(smem_u32(&ctl->acc_release[b]), 4);
+        }
+        ctl->abort_flag = 0;
+        fence_mbar_init();
+        fence_proxy_async_smem();
+    }
+    if (warp == 4) {
+        tmem_alloc(smem_u32(&ctl->tmem_base), S::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = ctl->tmem_base;
+    griddep_launch_dependents();   // after this CTA has its tensor memory: a CTA of the next kernel cannot take it away
+    if (!(warp == 5 && p.weights_early)) griddep_wait();
+
+    float sum[kFp8 ? kTokens : 1];      // Few8: this lane's weight row, all tokens
+    bool ok = true;
+    if (warp == 5 || warp == 6) {
+        // ------------------------------ loads
+        uint32_t s = 0, ph = 0;
+        for (int i = 0; i < count; ++i) {
+            ok = mbar_wait<true>(smem_u32(&ctl->empty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense);
+            if (kFp8 && warp == 6 && ok)
+                ok = mbar_wait<true>(smem_u32(&ctl->sempty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const uint32_t dst = smem_base + s * S::kStageBytes;
+            const int k0 = (begin + i) * (kFp8 ? 128 : 64);
+            if (warp == 5) {
+                const uint32_t bar = smem_u32(&ctl->wfull[s]);
+                mbar_arrive_expect_tx_elect(bar, S::kWeightBytes);
+                tma_load_2d_elect(dst, &p.w[0], bar, k0, w_row);
+                if constexpr (!kFp8) tma_load_2d_elect(dst + 16384, &p.w[1], bar, k0, w_row);
+            } else {
+                const uint32_t bar = smem_u32(&ctl->tfull[s]);
+                mbar_arrive_expect_tx_elect(bar, S::kTokenBytes);
+                tma_load_2d_elect(dst + S::kWeightBytes, &p.x, bar, k0, token0);
+                if constexpr (kFp8) {
+#pragma unroll
+                    for (int t = lane; t < kTokens; t += 32) {
+                        const bool valid = token0 + t < p.m;
+                        const float* src = valid ? p.sfa + (token0 + t) * p.sfa_row + (begin + i) * p.sfa_col : p.sfa;
+                        cp_async_4(smem_u32(&ctl->scale[s][t]), src, valid);
+                    }
+                    cp_async_arrive_noinc(smem_u32(&ctl->sfull[s]));
+                }
+            }
+            if (++s == kStages) { s = 0; ph ^= 1u; }
+        }
+        if (kFp8 && warp == 6) asm volatile("cp.async.wait_all;" ::: "memory");
+        if (!ok)
+            for (int i = 0; i < 64; ++i) __nanosleep(2000);   // error path: let copies in flight land
+        __syncwarp();
+    } else if (warp == 4) {
+        // ------------------------------ MMA issuer
+        constexpr uint32_t kIdesc = idesc_dense(128, kTokens, kFp8 ? 0u : (kBf16 ? 1u : 0u), false, false);
+        uint32_t s = 0, ph = 0;
+        for (int i = 0; i < count; ++i) {
+            ok = mbar_wait<true>(smem_u32(&ctl->wfull[s]), ph, abort_flag, p.status, kStatusDense) &&
+                 mbar_wait<true>(smem_u32(&ctl->tfull[s]), ph, abort_flag, p.status, kStatusDense);
+            if (kFp8 && ok && i >= 2)
+                ok = mbar_wait<true>(smem_u32(&ctl->acc_release[i & 1]), ((i >> 1) - 1) & 1, abort_flag, p.status, kStatusDense);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint32_t w = dense_desc_lo<false>(smem_base + s * S::kStageBytes);
+            const uint32_t t = w + (S::kWeightBytes >> 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (kFp8) {
+                    tc_mma_f8_one(tmem_base + (i & 1) * kTokens, w + 2 * j, t + 2 * j, kIdesc, j > 0 ? 1u : 0u);
+                } else {
+                    const uint32_t more = (i > 0 || j > 0) ? 1u : 0u;
+                    tc_mma_f16_one(tmem_base, w + 2 * j, t + 2 * j, kIdesc, more);
+                    tc_mma_f16_one(tmem_base + kTokens, w + (16384u >> 4) + 2 * j, t + 2 * j, kIdesc, more);
+                }
+            }
+            if constexpr (kFp8) tc_commit_elect(smem_u32(&ctl->acc_full[i & 1]));
+            tc_commit_elect(smem_u32(&ctl->empty[s]));
+            if (++s == kStages) { s = 0; ph ^= 1u; }
+        }
+        if constexpr (!kFp8)
+            if (ok) tc_commit_elect(smem_u32(&ctl->acc_full[0]));
+        __syncwarp();
+    } else if constexpr (kFp8) {
+        // ------------------------------ sums of the blocks
+        uint64_t acc[kTokens / 2];
+#pragma unroll
+        for (int j = 0; j < kTokens / 2; ++j) acc[j] = 0;
+        const bool exists = w_row < p.n;
+        const float* sb = p.sfb + (w_row / kFp8Block) * p.sfb_row + begin * p.sfb_col;
+        float b_next = exists && count > 0 ? sb[0] : 0.0f;
+        const uint32_t lanes = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
+        uint32_t s = 0, ph = 0;
+        for (int i = 0; i < count; ++i) {
+            const uint64_t b2 = pack_f32x2(__float_as_uint(b_next), __float_as_uint(b_next));
+            if (i + 1 < count) b_next = sb[(i + 1) * p.sfb_col];
+            ok = mbar_wait<true>(smem_u32(&ctl->sfull[s]), ph, abort_flag, p.status, kStatusDense) &&
+                 mbar_wait<true>(smem_u32(&ctl->acc_full[i & 1]), (i >> 1) & 1, abort_flag, p.status, kStatusDense);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint32_t scales = smem_u32(&ctl->scale[s][0]);
+#pragma unroll
+            for (int c = 0; c < kTokens / kChunk; ++c) {
+                uint32_t v[kChunk];
+                tc_ld_cols<kChunk>(lanes + (i & 1) * kTokens + c * kChunk, v);
+                tc_wait_ld();
+#pragma unroll
+                for (int j = 0; j < kChunk / 4; ++j) {
+                    uint32_t f0, f1, f2, f3;
+                    ld_shared_v4(scales + (c * kChunk + 4 * j) * 4, f0, f1, f2, f3);
+                    fma_f32x2(acc[c * (kChunk / 2) + 2 * j], pack_f32x2(v[4 * j], v[4 * j + 1]), mul_f32x2(pack_f32x2(f0, f1), b2));
+                    fma_f32x2(acc[c * (kChunk / 2) + 2 * j + 1], pack_f32x2(v[4 * j + 2], v[4 * j + 3]),
+                              mul_f32x2(pack_f32x2(f2, f3), b2));
+                }
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(smem_u32(&ctl->acc_release[i & 1]));
+                mbar_arrive(smem_u32(&ctl->sempty[s]));
+            }
+            if (++s == kStages) { s = 0; ph ^= 1u; }
+        }
+#pragma unroll
+        for (int j = 0; j < kTokens / 2; ++j) {
+            sum[2 * j] = __uint_as_float(static_cast<uint32_t>(acc[j]));
+            sum[2 * j + 1] = __uint_as_float(static_cast<uint32_t>(acc[j] >> 32));
+        }
+    } else {
+        ok = __all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->acc_full[0]), 0, abort_flag, p.status, kStatusDense));
+        tc_fence_after_sync();
+    }
+
+    // ------------------------------ results
+    const int tokens = p.m - token0 < kTokens ? p.m - token0 : kTokens;
+    const int row = w_row + warp * 32 + lane;                       // consumers: this lane's weight row = column of C
+    const uint32_t area = smem_base + (warp * 32 + lane) * 4;       // exchange: [g | u][token][128 rows]
+    uint16_t* out = p.c + token0 * p.ldc + row;
+    if (splits == 1) {
+        if (warp < 4 && ok) {
+            if constexpr (kFp8) {
+#pragma unroll
+                for (int t = 0; t < kTokens; ++t)
+                    if (t < tokens && row < p.n) out[t * p.ldc] = to_16<kBf16>(sum[t]);
+            } else {
+                const uint32_t acc = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
+#pragma unroll 1
+                for (int c = 0; c < kTokens / 16; ++c) {
+                    uint32_t g[16], u[16];
+                    tc_ld_x16(acc + c * 16, g);
+                    tc_ld_x16(acc + kTokens + c * 16, u);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int t = 0; t < 16; ++t)
+                        if (c * 16 + t < tokens && row < p.n)
+                            out[(c * 16 + t) * p.ldc] =
+                                to_16<kBf16>(gate<false>(__uint_as_float(g[t]), p.gelu).value * __uint_as_float(u[t]));
+                }
+            }
+        }
+    } else {
+        // every stage has been consumed (the last accumulator is complete): its memory now holds the partial sums
+        if (warp < 4 && ok) {
+            if constexpr (kFp8) {
+#pragma unroll
+                for (int t = 0; t < kTokens; ++t)
+                    if (t < tokens) st_shared_f32(area + t * 512, sum[t]);
+            } else {
+                const uint32_t acc = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
+#pragma unroll 1
+                for (int c = 0; c < kTokens / 16; ++c) {
+                    uint32_t g[16], u[16];
+                    tc_ld_x16(acc + c * 16, g);
+                    tc_ld_x16(acc + kTokens + c * 16, u);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int t = 0; t < 16; ++t)
+                        if (c * 16 + t < tokens) {
+                            st_shared_f32(area + (c * 16 + t) * 512, __uint_as_float(g[t]));
+                            st_shared_f32(area + (kTokens + c * 16 + t) * 512, __uint_as_float(u[t]));
+                        }
+                }
+            }
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (warp < 4 && row < p.n) {
+            // token t is summed by rank t % splits, in rank order
+            for (int t = rank; t < tokens; t += splits) {
+                float g = 0.0f, u = 0.0f;
+#pragma unroll 1
+                for (uint32_t r = 0; r < splits; ++r) {
+                    g += ld_cluster_f32(map_to_cta(area + t * 512, r));
+                    if constexpr (!kFp8) u += ld_cluster_f32(map_to_cta(area + (kTokens + t) * 512, r));
+                }
+                out[t * p.ldc] = to_16<kBf16>(kFp8 ? g : gate<false>(g, p.gelu).value * u);
+            }
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();            // nobody leaves while its sums are read
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 4) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, S::kTmemCols);
+    }
+}
+
+}  // namespace b200

@@ -94,8 +94,8 @@ template <bool kBf16, bool kPow2, bool kVec>
 __global__ void __launch_bounds__(kRowThreads)
 fp8_quantize_rows(const uint16_t* __restrict__ x, long long ldx, int rows, int k, uint8_t* __restrict__ q, long long ldq,
                   float* __restrict__ sf, long long sf_row, long long sf_col) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();   // in this order: whoever starts from here on finds all work before this kernel complete
     const int blocks_k = (k + kFp8Block - 1) / kFp8Block;
     const long long units = static_cast<long long>(rows) * blocks_k;
     const int half = threadIdx.x >> 4, l = threadIdx.x & 15;

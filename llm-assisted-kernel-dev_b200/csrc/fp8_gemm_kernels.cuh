@@ -54,7 +54,6 @@ fp8_gemm_pair(const __grid_constant__ Fp8Problem p) {
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int tiles = p.m_tiles * p.n_tiles;
     volatile uint32_t* abort_flag = &ctl->abort_flag;
-    griddep_launch_dependents();
     if (threadIdx.x == 0) {
         for (int s = 0; s < kFp8Stages; ++s) {
             mbar_init(smem_u32(&ctl->full[s]), 1);
@@ -79,6 +78,7 @@ fp8_gemm_pair(const __grid_constant__ Fp8Problem p) {
     cluster_arrive();
     cluster_wait();            // both CTAs' barriers exist
     const uint32_t tmem_base = ctl->tmem_base;
+    griddep_launch_dependents();   // after this CTA has its tensor memory: a CTA of the next kernel cannot take it away
     griddep_wait();
 
     if (warp == 9) {

@@ -209,7 +209,6 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
     const int tiles = p.m_tiles * p.n_tiles * p.batches;
     const int steps = p.k_tiles * p.segments;
     volatile uint32_t* abort_flag = &ctl->abort_flag;
-    griddep_launch_dependents();
     if (threadIdx.x == 0) {
         for (int s = 0; s < kFfStages; ++s) {
             mbar_init(smem_u32(&ctl->full[s]), 1);
@@ -234,6 +233,7 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
     cluster_arrive();
     cluster_wait();            // both CTAs' barriers exist
     const uint32_t tmem_base = ctl->tmem_base;
+    griddep_launch_dependents();   // after this CTA has its tensor memory: a CTA of the next kernel cannot take it away
     griddep_wait();
 
     if (warp == 5) {

@@ -14,26 +14,31 @@ from . import _lib
 
 E4M3 = torch.float8_e4m3fn
 BLOCK = 128
+_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+
+
+def _raw_stream(device_index: int) -> int:
+    """cudaStream_t of the device's current stream."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 def _dtype_code(dtype: torch.dtype, name: str) -> int:
-    if dtype == torch.bfloat16:
-        return _lib.DTYPE_BF16
-    if dtype == torch.float16:
-        return _lib.DTYPE_F16
-    raise ValueError(f"{name} must be float16 or bfloat16, got {dtype}")
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"{name} must be float16 or bfloat16, got {dtype}")
+    return code
 
 
 def _check_activations(x: torch.Tensor, what: str) -> None:
     if not x.is_cuda:
         raise ValueError(f"{what} needs a CUDA tensor (there is no CPU path)")
-    if x.dim() != 2 or x.shape[1] == 0 or (x.shape[1] > 1 and x.stride(1) != 1):
+    if x.dim() != 2 or x.shape[1] == 0 or (x.stride(1) != 1 and x.shape[1] > 1):
         raise ValueError(f"{what}: expected a matrix [rows, k >= 1] with unit stride along k")
 
 
 def _row_pitch(t: torch.Tensor) -> int:
-    """Row pitch in elements; a single row may carry any stride."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    """Row pitch in elements; the stride of a single row means nothing."""
+    return t.stride(0) if t.shape[0] > 1 else _padded(t.shape[1], 16)
 
 
 def _padded(n: int, to: int) -> int:
@@ -63,7 +68,7 @@ def quantize_fp8(x: torch.Tensor, *, pow2: bool = False):
         return q, sf
     code = _lib.load().b200_fp8_quantize_rows(x.data_ptr(), dtype, rows, k, _row_pitch(x), q.data_ptr(), _row_pitch(q),
                                               sf.data_ptr(), 1, rows, 1 if pow2 else 0,
-                                              torch.cuda.current_stream(x.device).cuda_stream, x.device.index)
+                                              _raw_stream(x.device.index), x.device.index)
     _lib.check(code)
     return q, sf
 
@@ -81,7 +86,7 @@ def quantize_fp8_weight(w: torch.Tensor):
     sf = torch.empty((-(-n // BLOCK), -(-k // BLOCK)), dtype=torch.float32, device=w.device)
     code = _lib.load().b200_fp8_quantize_blocks(w.data_ptr(), dtype, n, k, _row_pitch(w), q.data_ptr(), _row_pitch(q),
                                                 sf.data_ptr(), sf.stride(0), sf.stride(1),
-                                                torch.cuda.current_stream(w.device).cuda_stream, w.device.index)
+                                                _raw_stream(w.device.index), w.device.index)
     _lib.check(code)
     return q, sf
 
@@ -95,7 +100,7 @@ def dequantize_fp8(q: torch.Tensor, sf: torch.Tensor, dtype: torch.dtype = torch
     if rows:
         _lib.check(_lib.load().b200_fp8_dequantize_rows(q.data_ptr(), _row_pitch(q), sf.data_ptr(), sf.stride(0), sf.stride(1),
                                                         rows, k, code, out.data_ptr(), k,
-                                                        torch.cuda.current_stream(q.device).cuda_stream, q.device.index))
+                                                        _raw_stream(q.device.index), q.device.index))
     return out
 
 
@@ -148,7 +153,7 @@ def fp8_gemm(a: torch.Tensor, sfa: torch.Tensor, b: torch.Tensor, sfb: torch.Ten
         return out
     code = _lib.load().b200_fp8_gemm(a.data_ptr(), _row_pitch(a), sfa.data_ptr(), sfa.stride(0), sfa.stride(1), b.data_ptr(),
                                      _row_pitch(b), sfb.data_ptr(), sfb.stride(0), sfb.stride(1), out.data_ptr(),
-                                     _row_pitch(out), dtype, m, n, k, torch.cuda.current_stream(a.device).cuda_stream,
+                                     _row_pitch(out), dtype, m, n, k, _raw_stream(a.device.index),
                                      a.device.index, None)
     _lib.check(code)
     return out
@@ -165,9 +170,26 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_sf: torch.Tensor, *
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("fp8_linear has no backward pass: call it under torch.no_grad() or with a detached input")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    q, sf = quantize_fp8(x2)
-    out2 = out if out is None or out.dim() == 2 else out.view(-1, out.shape[-1])
-    y = fp8_gemm(q, sf, weight, weight_sf, out=out2, out_dtype=x.dtype)
+    _check_activations(x2, "fp8_linear")
+    dtype = _dtype_code(x.dtype, "x")
+    m, k = x2.shape
+    n = weight.shape[0]
+    device = x.device
+    _check_weight(weight, weight_sf, k, device, "fp8_linear")
+    y = torch.empty((m, n), dtype=x.dtype, device=device) if out is None else out if out.dim() == 2 else out.view(-1, out.shape[-1])
+    if out is not None:
+        _check_out(y, m, n, device, "fp8_linear")
+        if out.dtype != x.dtype:
+            raise ValueError(f"fp8_linear: out must be {x.dtype}, got {out.dtype}")
+    if m:
+        nbytes = m * _padded(k, 16) + 4 * m * -(-k // BLOCK)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        code = _lib.load().b200_fp8_linear(x2.data_ptr(), _row_pitch(x2), dtype, weight.data_ptr(), _row_pitch(weight),
+                                           weight_sf.data_ptr(), weight_sf.stride(0), weight_sf.stride(1), y.data_ptr(),
+                                           _row_pitch(y), m, n, k, scratch.data_ptr(), nbytes, _raw_stream(device.index),
+                                           device.index, None)
+        if code:
+            _lib.check(code)
     if out is not None:
         return out
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[1])
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], n)

@@ -43,7 +43,8 @@ def _check(x, w1, w2, activation, keep="inputs"):
 
 
 def _stream(t: torch.Tensor):
-    return torch.cuda.current_stream(t.device).cuda_stream, t.device.index
+    index = t.device.index
+    return fp8._raw_stream(index), index
 
 
 def _mat(t: torch.Tensor):
