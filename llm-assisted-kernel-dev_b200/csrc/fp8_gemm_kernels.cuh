@@ -32,7 +32,11 @@ constexpr int kFp8Stages = 6;
 constexpr uint32_t kFp8OperandBytes = 128u * 128u;
 constexpr uint32_t kFp8StageBytes = 2u * kFp8OperandBytes;
 constexpr uint32_t kFp8StagingBytes = 8u * 4096u;
-constexpr int kFp8Threads = 320;
+constexpr int kFp8Threads = 384;     // warps 10 and 11 only complete the third warpgroup's register hand-back
+// Registers: 384 threads start with 168 each; two promotion warpgroups take 216, the third keeps 72 (256 * 216 + 128 * 72 =
+// 384 * 168).
+constexpr uint32_t kFp8PromoteRegs = 216, kFp8OtherRegs = 72;
+static_assert(256 * kFp8PromoteRegs + 128 * kFp8OtherRegs <= 384 * 168, "register split");
 
 struct Fp8Control {
     uint64_t full[kFp8Stages], empty[kFp8Stages];
@@ -81,7 +85,9 @@ fp8_gemm_pair(const __grid_constant__ Fp8Problem p) {
     griddep_launch_dependents();   // after this CTA has its tensor memory: a CTA of the next kernel cannot take it away
     griddep_wait();
 
-    if (warp == 9) {
+    if (warp >= 8) {
+      warpgroup_reg_dec<kFp8OtherRegs>();
+      if (warp == 9) {
         // ------------------------------ producer: this CTA's 128 rows of A and of B
         uint32_t s = 0, ph = 0;
         bool ok = true;
@@ -104,7 +110,7 @@ fp8_gemm_pair(const __grid_constant__ Fp8Problem p) {
         if (!ok)
             for (int i = 0; i < 64; ++i) __nanosleep(2000);   // error path: let copies in flight land
         __syncwarp();
-    } else if (warp == 8) {
+      } else if (warp == 8) {
         // ------------------------------ MMA issuer
         if (rank == 0) {
             constexpr uint32_t kIdesc = idesc_dense(256, 256, 0u, false, false);
@@ -133,7 +139,9 @@ fp8_gemm_pair(const __grid_constant__ Fp8Problem p) {
             mbar_wait<true>(smem_u32(&ctl->done), 0, abort_flag, p.status, kStatusDense);
         }
         __syncwarp();
+      }
     } else {
+        warpgroup_reg_inc<kFp8PromoteRegs>();
         // ------------------------------ promotion and epilogue: 32 rows x 128 columns per warp, one row per lane
         const int quad = warp & 3, half = warp >> 2;
         BoxWriter<1> w{smem_base + kFp8Stages * kFp8StageBytes + static_cast<uint32_t>(warp) * 4096u, lane, 0};
@@ -158,24 +166,29 @@ fp8_gemm_pair(const __grid_constant__ Fp8Problem p) {
                     a_next = sa[(i + 1) * p.sfa_col];
                     b_next = sb[(i + 1) * p.sfb_col];
                 }
-                if (!__all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->acc_full[cnt & 1]), (cnt >> 1) & 1, abort_flag,
-                                                       p.status, kStatusDense))) {
+                if (!mbar_wait_warp(smem_u32(&ctl->acc_full[cnt & 1]), (cnt >> 1) & 1, lane, abort_flag, p.status, kStatusDense)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after_sync();
+                // the next 32 columns are on their way while these are added
+                const uint32_t src = lane_base + (cnt & 1) * 256;
+                uint32_t v[2][32];
+                tc_ld_x32(src, v[0]);
+                tc_wait_ld();
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    uint32_t v[32];
-                    tc_ld_x32(lane_base + (cnt & 1) * 256 + c * 32, v);
-                    tc_wait_ld();
-                    if (c == 3) {                        // everything read: the buffer goes back
+                    if (c < 3) {
+                        tc_ld_x32(src + (c + 1) * 32, v[(c + 1) & 1]);
+                    } else {                             // everything read: the buffer goes back
                         tc_fence_before_sync();
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&ctl->acc_release[cnt & 1]), 0));
                     }
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) fma_f32x2(acc[c * 16 + j], pack_f32x2(v[2 * j], v[2 * j + 1]), scale);
+                    for (int j = 0; j < 16; ++j)
+                        fma_f32x2(acc[c * 16 + j], pack_f32x2(v[c & 1][2 * j], v[c & 1][2 * j + 1]), scale);
+                    if (c < 3) tc_wait_ld();
                 }
             }
             if (!ok) break;
