@@ -61,14 +61,6 @@ template <FewOp kOp, int kTokens> constexpr uint32_t few_smem_bytes() {
 }
 constexpr int kFewThreads = 224;
 
-// 4-byte asynchronous copy (zero when not valid) and an arrival when this thread's copies so far have landed.
-__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool valid) {
-    const int bytes = valid ? 4 : 0;
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_arrive_noinc(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
-}
 __device__ __forceinline__ float4 ld_cluster_v4f(uint32_t cluster_addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -82,9 +74,6 @@ __device__ __forceinline__ void add_v4f(float4& a, const float4& b) {
     a.y += b.y;
     a.z += b.z;
     a.w += b.w;
-}
-__device__ __forceinline__ void st_shared_f32(uint32_t addr, float v) {
-    asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 template <bool kBf16> __device__ __forceinline__ uint16_t to_16(float v) { return static_cast<uint16_t>(pack_16<kBf16>(v, 0.0f)); }
 
@@ -252,8 +241,9 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
         }
 #pragma unroll
         for (int j = 0; j < kTokens / 2; ++j) {
-            sum[2 * j] = __uint_as_float(static_cast<uint32_t>(acc[j]));
-            sum[2 * j + 1] = __uint_as_float(static_cast<uint32_t>(acc[j] >> 32));
+            const float2 two = unpack_f32x2(acc[j]);
+            sum[2 * j] = two.x;
+            sum[2 * j + 1] = two.y;
         }
     } else {
         ok = __all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->acc_full[0]), 0, abort_flag, p.status, kStatusDense));

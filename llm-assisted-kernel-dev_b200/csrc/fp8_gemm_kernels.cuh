@@ -11,7 +11,8 @@
 // clock and SM); meanwhile the eight promotion warps of each SM read the 128 x 256 sums of the block before
 // (tensor memory, two buffers of 256 columns) and add them, scaled, to 128 registers per thread with packed
 // fp32 pairs: 64 fma.f32x2 per thread and block, 128 issue slots per scheduler.
-// Ten warps: 0-7 promotion and epilogue (quadrant w % 4, columns 128 (w / 4) ..), 8 MMA issuer, 9 TMA producer.
+// Twelve warps: 0-7 promotion and epilogue (quadrant w % 4, columns 128 (w / 4) ..), 8 MMA issuer, 9 TMA producer,
+// 10 scale products.
 #pragma once
 
 #include "dense_tiles.cuh"
@@ -28,10 +29,11 @@ struct Fp8Problem {
     uint32_t* status;
 };
 
-constexpr int kFp8Stages = 6;
+constexpr int kFp8Stages = 4;
+constexpr int kFp8Batch = 8;             // blocks whose scales are handed over at a time
 constexpr uint32_t kFp8OperandBytes = 128u * 128u;
 constexpr uint32_t kFp8StageBytes = 2u * kFp8OperandBytes;
-constexpr uint32_t kFp8StagingBytes = 8u * 4096u;
+constexpr uint32_t kFp8StagingBytes = 8u * 8192u;            // per promotion warp two boxes of 32 rows x 128 bytes
 constexpr int kFp8Threads = 384;     // warps 10 and 11 only complete the third warpgroup's register hand-back
 // Registers: 384 threads start with 168 each; two promotion warpgroups take 216, the third keeps 72 (256 * 216 + 128 * 72 =
 // 384 * 168).
@@ -40,10 +42,14 @@ static_assert(256 * kFp8PromoteRegs + 128 * kFp8OtherRegs <= 384 * 168, "registe
 
 struct Fp8Control {
     uint64_t full[kFp8Stages], empty[kFp8Stages];
-    uint64_t acc_full[2], acc_release[2], done;
+    uint64_t acc_full[2], acc_release[2], scale_full[2], scale_free[2], done;
     uint32_t tmem_base, abort_flag;
+    int2 place[4];               // row and column of the tiles whose scales are in the ring
 };
-constexpr uint32_t kFp8SmemBytes = 1024u + kFp8Stages * kFp8StageBytes + kFp8StagingBytes + sizeof(Fp8Control);
+// scale products: two batches of kFp8Batch blocks x [column half][128 rows]
+constexpr uint32_t kFp8BatchBytes = kFp8Batch * 2u * 128u * 4u;
+constexpr uint32_t kFp8RingBytes = 2u * kFp8BatchBytes;
+constexpr uint32_t kFp8SmemBytes = 1024u + kFp8Stages * kFp8StageBytes + kFp8StagingBytes + kFp8RingBytes + sizeof(Fp8Control);
 static_assert(kFp8SmemBytes <= 227u * 1024u, "shared memory budget");
 
 template <bool kBf16>
@@ -52,11 +58,10 @@ fp8_gemm_pair(const __grid_constant__ Fp8Problem p) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     Fp8Control* ctl = reinterpret_cast<Fp8Control*>(smem_raw + (smem_base - smem_u32(smem_raw)) +
-                                                    kFp8Stages * kFp8StageBytes + kFp8StagingBytes);
+                                                    kFp8Stages * kFp8StageBytes + kFp8StagingBytes + kFp8RingBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_cta_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-    const int tiles = p.m_tiles * p.n_tiles;
     volatile uint32_t* abort_flag = &ctl->abort_flag;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kFp8Stages; ++s) {
@@ -66,6 +71,8 @@ fp8_gemm_pair(const __grid_constant__ Fp8Problem p) {
         for (int b = 0; b < 2; ++b) {
             mbar_init(smem_u32(&ctl->acc_full[b]), 1);
             mbar_init(smem_u32(&ctl->acc_release[b]), 16);   // eight promotion warps of each CTA; used in the first
+            mbar_init(smem_u32(&ctl->scale_full[b]), 32);    // every lane of the scale warp
+            mbar_init(smem_u32(&ctl->scale_free[b]), 8);     // the promotion warps
         }
         mbar_init(smem_u32(&ctl->done), 1);
         ctl->abort_flag = 0;
@@ -91,8 +98,7 @@ fp8_gemm_pair(const __grid_constant__ Fp8Problem p) {
         // ------------------------------ producer: this CTA's 128 rows of A and of B
         uint32_t s = 0, ph = 0;
         bool ok = true;
-        for (int tile = pair; ok && tile < tiles; tile += pairs) {
-            const TileAt t = banded_tile(tile, p.m_tiles, p.n_tiles);
+        for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, 1); ok && t.valid(); t.next()) {
             const int a_row = t.m * 256 + static_cast<int>(rank) * 128, b_row = t.n * 256 + static_cast<int>(rank) * 128;
             for (int i = 0; i < p.k_tiles; ++i) {
                 if (!__all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->empty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense))) {
@@ -110,19 +116,60 @@ fp8_gemm_pair(const __grid_constant__ Fp8Problem p) {
         if (!ok)
             for (int i = 0; i < 64; ++i) __nanosleep(2000);   // error path: let copies in flight land
         __syncwarp();
+      } else if (warp == 10) {
+        // ------------------------------ scales: products s_A s_B of this CTA's 128 rows and both column halves
+        const uint32_t ring = smem_base + kFp8Stages * kFp8StageBytes + kFp8StagingBytes;
+        uint32_t batch = 0, nth = 0;
+        bool ok = true;
+        for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, 1); ok && t.valid(); t.next(), ++nth) {
+            const int row0 = t.m * 256 + static_cast<int>(rank) * 128, col = t.n * 256;
+            // rows and columns past the matrix get scales that exist; what they scale is never stored
+            const float* sa[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sa[r] = p.sfa + (row0 + r * 32 + lane < p.m ? row0 + r * 32 + lane : 0) * p.sfa_row;
+            const float* sb = p.sfb + (col / kFp8Block) * p.sfb_row;
+            const long long next_half = col + 128 < p.n ? p.sfb_row : 0;
+            for (int i0 = 0; i0 < p.k_tiles; i0 += kFp8Batch, ++batch) {
+                ok = mbar_wait_converged(smem_u32(&ctl->scale_free[batch & 1]), ((batch >> 1) & 1) ^ 1u, abort_flag, p.status, kStatusDense);
+                if (!ok) break;
+                if (i0 == 0 && lane == 0) ctl->place[nth & 3] = make_int2(row0, col);
+                const uint32_t dst = ring + (batch & 1) * kFp8BatchBytes + lane * 4;
+#pragma unroll
+                for (int part = 0; part < kFp8Batch; part += 4) {
+                    float a[4][4], b[4][2];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int at = i0 + part + j < p.k_tiles ? i0 + part + j : p.k_tiles - 1;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) a[j][r] = sa[r][at * p.sfa_col];
+                        b[j][0] = sb[at * p.sfb_col];
+                        b[j][1] = sb[at * p.sfb_col + next_half];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            st_shared_f32(dst + (part + j) * 1024 + r * 128, a[j][r] * b[j][0]);
+                            st_shared_f32(dst + (part + j) * 1024 + 512 + r * 128, a[j][r] * b[j][1]);
+                        }
+                }
+                mbar_arrive(smem_u32(&ctl->scale_full[batch & 1]));
+            }
+        }
+        __syncwarp();
       } else if (warp == 8) {
         // ------------------------------ MMA issuer
         if (rank == 0) {
             constexpr uint32_t kIdesc = idesc_dense(256, 256, 0u, false, false);
             uint32_t s = 0, ph = 0, cnt = 0;
             bool ok = true;
-            for (int tile = pair; ok && tile < tiles; tile += pairs) {
+            for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, 1); ok && t.valid(); t.next()) {
 #pragma unroll 1
                 for (int i = 0; i < p.k_tiles; ++i, ++cnt) {
-                    ok = mbar_wait<true>(smem_u32(&ctl->full[s]), ph, abort_flag, p.status, kStatusDense);
+                    ok = mbar_wait_converged(smem_u32(&ctl->full[s]), ph, abort_flag, p.status, kStatusDense);
                     if (ok && cnt >= 2)
-                        ok = mbar_wait<true>(smem_u32(&ctl->acc_release[cnt & 1]), ((cnt >> 1) - 1) & 1, abort_flag, p.status, kStatusDense);
-                    ok = __all_sync(0xffffffffu, ok);
+                        ok = mbar_wait_converged(smem_u32(&ctl->acc_release[cnt & 1]), ((cnt >> 1) - 1) & 1, abort_flag, p.status,
+                                                 kStatusDense);
                     if (!ok) break;
                     tc_fence_after_sync();
                     const uint32_t a = dense_desc_lo<false>(smem_base + s * kFp8StageBytes);
@@ -144,54 +191,60 @@ fp8_gemm_pair(const __grid_constant__ Fp8Problem p) {
         warpgroup_reg_inc<kFp8PromoteRegs>();
         // ------------------------------ promotion and epilogue: 32 rows x 128 columns per warp, one row per lane
         const int quad = warp & 3, half = warp >> 2;
-        BoxWriter<1> w{smem_base + kFp8Stages * kFp8StageBytes + static_cast<uint32_t>(warp) * 4096u, lane, 0};
+        BoxWriter w{smem_base + kFp8Stages * kFp8StageBytes + static_cast<uint32_t>(warp) * 8192u, lane, 0};
         const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + half * 128;
-        uint32_t cnt = 0;
+        const uint32_t ring = smem_base + kFp8Stages * kFp8StageBytes + kFp8StagingBytes + half * 512 + (quad * 32 + lane) * 4;
+        const uint32_t scale_full = smem_u32(&ctl->scale_full[0]), scale_free = smem_u32(&ctl->scale_free[0]);
+        const uint32_t acc_full = smem_u32(&ctl->acc_full[0]), release = map_to_cta(smem_u32(&ctl->acc_release[0]), 0);
+        uint32_t cnt = 0, batch = 0;
         bool ok = true;
-        for (int tile = pair; ok && tile < tiles; tile += pairs) {
-            const TileAt t = banded_tile(tile, p.m_tiles, p.n_tiles);
-            const int row = t.m * 256 + static_cast<int>(rank) * 128 + quad * 32, col = t.n * 256 + half * 128;
-            const bool exists = row + lane < p.m && col < p.n;
-            const float* sa = p.sfa + (row + lane) * p.sfa_row;
-            const float* sb = p.sfb + (col / kFp8Block) * p.sfb_row;
-            float a_next = exists ? sa[0] : 0.0f, b_next = exists ? sb[0] : 0.0f;
+        // where a tile lies is only needed at its end: the scale warp, which walks the tiles, hands it over with the scales
+        const int mine = (p.m_tiles * p.n_tiles - pair + pairs - 1) / pairs;
+        for (int nth = 0; ok && nth < mine; ++nth) {
+            // the scale of block i, read while the block before is being added
+            auto next_scale = [&](int i) {
+                if (i % kFp8Batch == 0) {
+                    if (i > 0) mbar_arrive_elect(scale_free + 8 * (batch++ & 1));
+                    ok = mbar_wait_converged(scale_full + 8 * (batch & 1), (batch >> 1) & 1, abort_flag, p.status, kStatusDense);
+                }
+                const uint32_t f = ld_shared_u32(ring + (batch & 1) * kFp8BatchBytes + (i % kFp8Batch) * 1024);
+                return pack_f32x2(f, f);
+            };
             uint64_t acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0;
+            uint64_t scale = next_scale(0);
 #pragma unroll 1
-            for (int i = 0; i < p.k_tiles; ++i, ++cnt) {
-                const float f = a_next * b_next;
-                const uint64_t scale = pack_f32x2(__float_as_uint(f), __float_as_uint(f));
-                if (exists && i + 1 < p.k_tiles) {       // a block ahead: arrives while this one is worked on
-                    a_next = sa[(i + 1) * p.sfa_col];
-                    b_next = sb[(i + 1) * p.sfb_col];
-                }
-                if (!mbar_wait_warp(smem_u32(&ctl->acc_full[cnt & 1]), (cnt >> 1) & 1, lane, abort_flag, p.status, kStatusDense)) {
+            for (int i = 0; ok && i < p.k_tiles; ++i) {
+                const uint32_t buf = cnt & 1;
+                if (!mbar_wait_converged(acc_full + 8 * buf, (cnt >> 1) & 1, abort_flag, p.status, kStatusDense)) {
                     ok = false;
                     break;
                 }
+                ++cnt;
                 tc_fence_after_sync();
-                // the next 32 columns are on their way while these are added
-                const uint32_t src = lane_base + (cnt & 1) * 256;
-                uint32_t v[2][32];
-                tc_ld_x32(src, v[0]);
-                tc_wait_ld();
+                const uint32_t src = lane_base + buf * 256;
+                uint64_t scale_next = scale;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    if (c < 3) {
-                        tc_ld_x32(src + (c + 1) * 32, v[(c + 1) & 1]);
-                    } else {                             // everything read: the buffer goes back
+                    uint32_t v[32];
+                    tc_ld_x32(src + c * 32, v);
+                    tc_wait_ld();
+                    if (c == 3) {                        // everything read: the buffer goes back
                         tc_fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&ctl->acc_release[cnt & 1]), 0));
+                        mbar_arrive_cluster_relaxed_elect(release + 8 * buf);
                     }
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        fma_f32x2(acc[c * 16 + j], pack_f32x2(v[c & 1][2 * j], v[c & 1][2 * j + 1]), scale);
-                    if (c < 3) tc_wait_ld();
+                    for (int j = 0; j < 16; ++j) fma_f32x2(acc[c * 16 + j], pack_f32x2(v[2 * j], v[2 * j + 1]), scale);
+                    if (c == 1 && i + 1 < p.k_tiles) scale_next = next_scale(i + 1);
                 }
+                scale = scale_next;
             }
             if (!ok) break;
+            const int2 at = ctl->place[nth & 3];
+            const int row = at.x + quad * 32, col = at.y + half * 128;
+            __syncwarp();
+            mbar_arrive_elect(scale_free + 8 * (batch++ & 1));
 #pragma unroll
             for (int part = 0; part < 2; ++part) {
                 const uint32_t box = w.acquire();
@@ -200,8 +253,9 @@ fp8_gemm_pair(const __grid_constant__ Fp8Problem p) {
                     float f[32];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        f[2 * j] = __uint_as_float(static_cast<uint32_t>(acc[part * 32 + c * 16 + j]));
-                        f[2 * j + 1] = __uint_as_float(static_cast<uint32_t>(acc[part * 32 + c * 16 + j] >> 32));
+                        const float2 two = unpack_f32x2(acc[part * 32 + c * 16 + j]);
+                        f[2 * j] = two.x;
+                        f[2 * j + 1] = two.y;
                     }
                     put_chunk<kBf16>(w, box, c * 4, f);
                 }

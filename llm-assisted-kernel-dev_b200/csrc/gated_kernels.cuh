@@ -77,7 +77,7 @@ template <bool kSlope> __device__ __forceinline__ GateValue gate(float z, int ge
 
 // h = act(g) u of 32 rows x 128 columns.
 template <bool kBf16>
-__device__ __forceinline__ void ff_epilogue_forward(const FfProblem& p, uint32_t acc, BoxWriter<2>& w, int row, int col) {
+__device__ __forceinline__ void ff_epilogue_forward(const FfProblem& p, uint32_t acc, BoxWriter& w, int row, int col) {
 #pragma unroll 1
     for (int half = 0; half < 2; ++half) {
         const uint32_t box = w.acquire();
@@ -97,7 +97,7 @@ __device__ __forceinline__ void ff_epilogue_forward(const FfProblem& p, uint32_t
 }
 
 // 8-bit copy of one projection's 32 rows x 128 columns (a lane holds a whole block: its row's 128 columns).
-__device__ __forceinline__ void ff_epilogue_keep(const FfProblem& p, int which, uint32_t acc, BoxWriter<2>& w, int row, int col) {
+__device__ __forceinline__ void ff_epilogue_keep(const FfProblem& p, int which, uint32_t acc, BoxWriter& w, int row, int col) {
     float m = kAmaxFloor;
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
@@ -129,7 +129,7 @@ __device__ __forceinline__ void ff_epilogue_keep(const FfProblem& p, int which, 
 
 // dg and du of 32 rows x 128 columns from the accumulators and dh.
 template <bool kBf16>
-__device__ __forceinline__ void ff_epilogue_grad_hidden(const FfProblem& p, uint32_t acc, BoxWriter<2>& w, int row, int col) {
+__device__ __forceinline__ void ff_epilogue_grad_hidden(const FfProblem& p, uint32_t acc, BoxWriter& w, int row, int col) {
     const int r = row + w.lane;
     const uint16_t* dh = p.dh + r * p.ld_dh + col;
 #pragma unroll 1
@@ -173,7 +173,7 @@ __device__ __forceinline__ void ff_epilogue_grad_hidden(const FfProblem& p, uint
 
 // 32 rows x 256 columns of a plain product.
 template <bool kBf16>
-__device__ __forceinline__ void ff_epilogue_plain(const FfProblem& p, const CUtensorMap* map, uint32_t acc, BoxWriter<2>& w,
+__device__ __forceinline__ void ff_epilogue_plain(const FfProblem& p, const CUtensorMap* map, uint32_t acc, BoxWriter& w,
                                                   int row, int col) {
 #pragma unroll 1
     for (int part = 0; part < 4; ++part) {
@@ -206,7 +206,6 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_cta_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-    const int tiles = p.m_tiles * p.n_tiles * p.batches;
     const int steps = p.k_tiles * p.segments;
     volatile uint32_t* abort_flag = &ctl->abort_flag;
     if (threadIdx.x == 0) {
@@ -240,8 +239,7 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
         // ------------------------------ producer: this CTA's rows of A and its half of B
         uint32_t s = 0, ph = 0;
         bool ok = true;
-        for (int tile = pair; ok && tile < tiles; tile += pairs) {
-            const TileAt t = banded_tile(tile, p.m_tiles, p.n_tiles);
+        for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, p.batches); ok && t.valid(); t.next()) {
             const int a_row = t.m * 256 + static_cast<int>(rank) * 128;
             const int b_row = kDual ? t.n * 128 : t.n * 256 + static_cast<int>(rank) * 128;
             for (int i = 0; i < steps; ++i) {
@@ -281,7 +279,7 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
             uint32_t s = 0, ph = 0;
             int it = 0;
             bool ok = true;
-            for (int tile = pair; ok && tile < tiles; tile += pairs, ++it) {
+            for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, p.batches); ok && t.valid(); t.next(), ++it) {
                 if (it >= 2)
                     ok = __all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->acc_release[it & 1]), ((it >> 1) - 1) & 1, abort_flag,
                                                            p.status, kStatusDense));
@@ -311,10 +309,9 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
         __syncwarp();
     } else {
         // ------------------------------ epilogue
-        BoxWriter<2> w{smem_base + kFfStages * kFfStageBytes + static_cast<uint32_t>(warp) * 8192u, lane, 0};
+        BoxWriter w{smem_base + kFfStages * kFfStageBytes + static_cast<uint32_t>(warp) * 8192u, lane, 0};
         int it = 0;
-        for (int tile = pair; tile < tiles; tile += pairs, ++it) {
-            const TileAt t = banded_tile(tile, p.m_tiles, p.n_tiles);
+        for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, p.batches); t.valid(); t.next(), ++it) {
             if (!__all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->acc_full[it & 1]), (it >> 1) & 1, abort_flag, p.status, kStatusDense)))
                 break;
             tc_fence_after_sync();

@@ -100,6 +100,74 @@ __device__ __forceinline__ void tc_commit_elect(uint32_t bar) {
         : "memory");
 }
 
+// Arrive (no release ordering, see mbar_arrive_cluster_relaxed) by one elected lane of a converged warp.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed_elect(uint32_t cluster_addr) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n\t"
+        "}\n" ::"r"(cluster_addr)
+        : "memory");
+}
+
+// Arrive on a barrier of this CTA (release) by one elected lane of a converged warp.
+__device__ __forceinline__ void mbar_arrive_elect(uint32_t bar) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e mbarrier.arrive.shared::cta.b64 _, [%0];\n\t"
+        "}\n" ::"r"(bar)
+        : "memory");
+}
+
+// Bounded wait of a converged warp in lock step: every lane tries, one vote decides, so a barrier that is already
+// complete costs no divergent branch (about 40 clocks against 350 when one lane polls inside an `if`).
+__device__ __forceinline__ bool mbar_wait_converged_slow(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                                      uint32_t* status, uint32_t code) {
+    const long long t0 = clock64();
+#pragma unroll 1
+    while (true) {
+#pragma unroll 1
+        for (int i = 0; i < 256; ++i)
+            if (__all_sync(0xffffffffu, mbar_try_wait_parked(bar, parity, 20000u))) return true;
+        if (__any_sync(0xffffffffu, *abort_flag != 0u || clock64() - t0 > kWaitTimeoutCycles)) {
+            if (*abort_flag == 0u) atomicOr(status, code);
+            *abort_flag = 1u;
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ bool mbar_wait_converged(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                                    uint32_t* status, uint32_t code) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    return mbar_wait_converged_slow(bar, parity, abort_flag, status, code);
+}
+
+__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_shared_f32(uint32_t addr, float v) {
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+// Asynchronous copies of four bytes into shared memory, completion per thread.
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool valid = true) {   // zero when not valid
+    const int bytes = valid ? 4 : 0;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending> __device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+// Arrival on an mbarrier when this thread's copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive_noinc(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 // TMEM -> registers, 32 consecutive columns of the warp's own lane quadrant.
 __device__ __forceinline__ void tc_ld_x32(uint32_t taddr, uint32_t* v) {
     asm volatile(
@@ -157,7 +225,14 @@ __device__ __forceinline__ uint64_t mul_f32x2(uint64_t x, uint64_t y) {
     return r;
 }
 __device__ __forceinline__ uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {
-    return static_cast<uint64_t>(lo) | (static_cast<uint64_t>(hi) << 32);
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
 }
 
 }  // namespace b200
