@@ -382,8 +382,9 @@ int b200_fp8_gemm(const void* a, int64_t lda, const float* sfa, int64_t sfa_row,
 /* b200_fp8_linear: y = values(quantised x) . values(w)^T in one call, x [m, k] fp16 or bf16 (row
  *   pitch ldx, any alignment), y of the same type; equals b200_fp8_quantize_rows (pow2 = 0)
  *   followed by b200_fp8_gemm bit for bit.  The weights start to load while x is quantised.
- *   scratch: b200_fp8_linear_scratch_bytes(m, k) bytes, 16-byte aligned, free again once the call's
- *   work on the stream is done. */
+ *   scratch: b200_fp8_linear_scratch_bytes(m, k) bytes (0, then NULL, up to 16 rows: these are
+ *   quantised inside the product's kernel), 16-byte aligned, free again once the call's work on
+ *   the stream is done. */
 size_t b200_fp8_linear_scratch_bytes(int m, int k);
 int b200_fp8_linear(const void* x, int64_t ldx, int dtype, const void* w, int64_t ldw,
                     const float* sfw, int64_t sfw_row, int64_t sfw_col, void* y, int64_t ldy, int m,
@@ -404,28 +405,26 @@ int b200_fp8_linear(const void* x, int64_t ldx, int dtype, const void* w, int64_
 #define B200_ACT_SILU 0
 #define B200_ACT_GELU 1 /* tanh form */
 
-/* h; with qg != NULL also 8-bit copies of g and u (format above, pow2 scales, [m, n]) for
- * b200_gated_grad_hidden_kept. */
+/* h.  kept == NULL: nothing else.  Otherwise also, into one buffer of b200_gated_kept_bytes(m, n,
+ *   k, keep_x) bytes, 8-bit copies of g, u and (keep_x != 0) x in the format above with power-of-two
+ *   scales: codes of g, u, x (row pitches padded to 16 bytes), then the scales of g, u, x, those
+ *   of one 128-wide block of all rows side by side. */
+size_t b200_gated_kept_bytes(int m, int n, int k, int keep_x);
 int b200_gated_forward(const void* x, int64_t ldx, const void* w1, int64_t ldw1, const void* w2,
-                       int64_t ldw2, int dtype, int act, void* h, int64_t ldh, void* qg, void* qu,
-                       int64_t ldq, float* sg, float* su, int64_t sf_row, int64_t sf_col, int m,
-                       int n, int k, void* stream, int device, uint32_t* status);
-/* dg and du, with g and u formed again from x and the weights. */
-int b200_gated_grad_hidden(const void* x, int64_t ldx, const void* w1, int64_t ldw1, const void* w2,
-                           int64_t ldw2, int dtype, int act, const void* dh, int64_t ld_dh, void* dg,
-                           void* du, int64_t ld_out, int m, int n, int k, void* stream, int device,
-                           uint32_t* status);
-/* dg and du, with the values of the 8-bit copies for g and u. */
-int b200_gated_grad_hidden_kept(const void* qg, const void* qu, int64_t ldq, const float* sg,
-                                const float* su, int64_t sf_row, int64_t sf_col, int dtype, int act,
-                                const void* dh, int64_t ld_dh, void* dg, void* du, int64_t ld_out,
-                                int m, int n, void* stream, int device);
-int b200_gated_grad_input(const void* dg, const void* du, int64_t ld_g, const void* w1, int64_t ldw1,
-                          const void* w2, int64_t ldw2, int dtype, void* dx, int64_t ld_dx, int m,
-                          int n, int k, void* stream, int device, uint32_t* status);
-int b200_gated_grad_weight(const void* dg, const void* du, int64_t ld_g, const void* x, int64_t ldx,
-                           int dtype, void* dw1, void* dw2, int64_t ld_dw, int m, int n, int k,
-                           void* stream, int device, uint32_t* status);
+                       int64_t ldw2, int dtype, int act, void* h, int64_t ldh, void* kept,
+                       size_t kept_bytes, int keep_x, int m, int n, int k, void* stream, int device,
+                       uint32_t* status);
+/* dx, dw1, dw2 (each NULL if not wanted, one at least is) from dh.  kept == NULL: g and u are
+ *   formed again from x and the weights.  Otherwise the values of the 8-bit copies stand for g, u
+ *   and x, and x is not read; keep_x says whether x is among them, as dw1 and dw2 need it.  scratch:
+ *   b200_gated_backward_scratch_bytes(m, n, k, kept != NULL) bytes, 16-byte aligned, free again
+ *   once the call's work on the stream is done. */
+size_t b200_gated_backward_scratch_bytes(int m, int n, int k, int kept);
+int b200_gated_backward(const void* x, int64_t ldx, const void* kept, size_t kept_bytes,
+                        int keep_x, const void* w1, int64_t ldw1, const void* w2, int64_t ldw2, int dtype, int act,
+                        const void* dh, int64_t ld_dh, void* dx, int64_t ld_dx, void* dw1, void* dw2,
+                        int64_t ld_dw, int m, int n, int k, void* scratch, size_t scratch_bytes,
+                        void* stream, int device, uint32_t* status);
 
 /* Synchronise `stream`, copy the library-owned status word of `device` into
  * *out and clear it. */

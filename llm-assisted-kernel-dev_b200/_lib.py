@@ -61,13 +61,11 @@ SIGNATURES = {
     "b200_fp8_gemm": (_i, [_vp, _i64, _vp, _i64, _i64] * 2 + [_vp, _i64] + [_i] * 4 + [_vp, _i, _vp]),
     "b200_fp8_linear_scratch_bytes": (_sz, [_i, _i]),
     "b200_fp8_linear": (_i, [_vp, _i64, _i, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i, _i, _i, _vp, _sz, _vp, _i, _vp]),
-    "b200_gated_forward": (_i, [_vp, _i64] * 3 + [_i, _i, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64] + [_i] * 3 +
-                           [_vp, _i, _vp]),
-    "b200_gated_grad_hidden": (_i, [_vp, _i64] * 3 + [_i, _i, _vp, _i64, _vp, _vp, _i64] + [_i] * 3 + [_vp, _i, _vp]),
-    "b200_gated_grad_hidden_kept": (_i, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _i, _i, _vp, _i64, _vp, _vp, _i64, _i, _i,
-                                         _vp, _i]),
-    "b200_gated_grad_input": (_i, [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _i, _vp, _i64] + [_i] * 3 + [_vp, _i, _vp]),
-    "b200_gated_grad_weight": (_i, [_vp, _vp, _i64, _vp, _i64, _i, _vp, _vp, _i64] + [_i] * 3 + [_vp, _i, _vp]),
+    "b200_gated_kept_bytes": (_sz, [_i] * 4),
+    "b200_gated_forward": (_i, [_vp, _i64] * 3 + [_i, _i, _vp, _i64, _vp, _sz] + [_i] * 4 + [_vp, _i, _vp]),
+    "b200_gated_backward_scratch_bytes": (_sz, [_i] * 4),
+    "b200_gated_backward": (_i, [_vp, _i64, _vp, _sz, _i, _vp, _i64, _vp, _i64, _i, _i] + [_vp, _i64] * 2 +
+                            [_vp, _vp, _i64] + [_i] * 3 + [_vp, _sz, _vp, _i, _vp]),
     "b200_read_status": (_i, [_i, _vp, _u32p]),
     "b200_read_last_cycles": (_i, [_i, _vp, ctypes.POINTER(ctypes.c_uint64)]),
     "b200_probe_l2_feed": (_i, [_i, _i, _i, _i, _i, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double),

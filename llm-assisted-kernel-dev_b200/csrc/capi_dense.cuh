@@ -61,6 +61,8 @@ struct DenseCall {
         if ((rc = opt_in_smem(fp8_gemm_pair<true>, kFp8SmemBytes))) return;
         if ((rc = opt_in_few_all<FewOp::Few8>())) return;
         if ((rc = opt_in_few_all<FewOp::FewGated>())) return;
+        if ((rc = opt_in_smem(few_tokens_gemm<FewOp::Few8, 16, false, true>, few_smem_bytes<FewOp::Few8, 16>()))) return;
+        if ((rc = opt_in_smem(few_tokens_gemm<FewOp::Few8, 16, true, true>, few_smem_bytes<FewOp::Few8, 16>()))) return;
         if ((rc = opt_in_ff<FfMode::Forward>())) return;
         if ((rc = opt_in_ff<FfMode::GradHidden>())) return;
         if ((rc = opt_in_ff<FfMode::GradInput>())) return;
@@ -140,14 +142,14 @@ int few_splits(long long tiles, int steps, int slots) {
     return s;
 }
 
-template <FewOp kOp, int kTokens, bool kBf16> int launch_few_as(FewProblem& p, DenseCall& call) {
+template <FewOp kOp, int kTokens, bool kBf16, bool kFuse = false> int launch_few_as(FewProblem& p, DenseCall& call) {
     using S = FewShape<kOp, kTokens>;
     const int tiles = (p.n + 127) / 128, token_tiles = (p.m + kTokens - 1) / kTokens;
     const int splits = few_splits(static_cast<long long>(tiles) * token_tiles, p.steps, call.st->sm_count * S::kCtasPerSm);
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
     cfg.gridDim = dim3(tiles * splits, token_tiles, 1);
-    cfg.blockDim = dim3(kFewThreads, 1, 1);
+    cfg.blockDim = dim3(kFuse ? kFewFuseThreads : kFewThreads, 1, 1);
     cfg.dynamicSmemBytes = few_smem_bytes<kOp, kTokens>();
     cfg.stream = call.stream;
     cudaLaunchAttribute attr[2];
@@ -159,7 +161,7 @@ template <FewOp kOp, int kTokens, bool kBf16> int launch_few_as(FewProblem& p, D
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    B200_CUDA(cudaLaunchKernelEx(&cfg, few_tokens_gemm<kOp, kTokens, kBf16>, p));
+    B200_CUDA(cudaLaunchKernelEx(&cfg, few_tokens_gemm<kOp, kTokens, kBf16, kFuse>, p));
     ++g_launches;
     g_last_kernel = kOp == FewOp::Few8 ? "few_tokens_gemm<Few8>" : "few_tokens_gemm<FewGated>";
     return 0;
@@ -177,6 +179,7 @@ template <FewOp kOp> int launch_few(FewProblem& p, int dtype, DenseCall& call, u
     }
 }
 constexpr int kFewMost = 256;
+constexpr int kFuseMost = 16;            // rows up to which fp8_linear quantises inside the product's kernel
 
 // Maps and sizes that the forward pass and its recomputation share.
 int ff_projections(FfProblem& p, const void* x, long long ldx, const void* w1, long long ldw1, const void* w2, long long ldw2,
@@ -201,7 +204,7 @@ int quantize_rows_launch(const char* what, const void* x, int dtype, int rows, i
     const long long units = static_cast<long long>(rows) * ((k + kFp8Block - 1) / kFp8Block);
     constexpr int kPerBlock = kRowThreads / 16 * kRowUnits;
     const long long blocks = (units + kPerBlock - 1) / kPerBlock;
-    if (blocks > 0x7FFFFFFFll) return fail(B200_E_LIMIT, "%s: %d rows and k=%d are too many blocks for one launch", what, rows, k);
+    if (units + kPerBlock > 0xFFFFFFFFll) return fail(B200_E_LIMIT, "%s: %d rows and k=%d are too many blocks", what, rows, k);
     const bool vec = aligned16(x) && ldx % 8 == 0;
     const uint16_t* src = static_cast<const uint16_t*>(x);
     uint8_t* qp = static_cast<uint8_t*>(q);
@@ -216,6 +219,38 @@ int quantize_rows_launch(const char* what, const void* x, int dtype, int rows, i
     if (pow2) return vec ? go(&fp8_quantize_rows<false, true, true>) : go(&fp8_quantize_rows<false, true, false>);
     return vec ? go(&fp8_quantize_rows<false, false, true>) : go(&fp8_quantize_rows<false, false, false>);
 }
+
+int dequantize_rows_launch(const char* what, const void* q, long long ldq, const float* sf, long long sf_row, long long sf_col,
+                           int rows, int k, int out_dtype, void* out, long long ldo, DenseCall& call) {
+    const long long blocks = (static_cast<long long>(rows) * ((k + 7) / 8) + 255) / 256;
+    if (blocks * 256 > 0xFFFFFFFFll) return fail(B200_E_LIMIT, "%s: %d rows and k=%d are too many", what, rows, k);
+    auto* kernel = out_dtype == B200_DTYPE_BF16 ? &fp8_dequantize_rows<true> : &fp8_dequantize_rows<false>;
+    return launch_dense("fp8_dequantize_rows", kernel, dim3(static_cast<unsigned>(blocks)), 256, 0u, call.stream,
+                        static_cast<const uint8_t*>(q), ldq, sf, sf_row, sf_col, rows, k, static_cast<uint16_t*>(out), ldo);
+}
+
+// What the gated block keeps in 8 bits, one buffer: codes of g, u [m, n] and, on request, x [m, k] (row pitches padded to
+// 16 bytes), then their power-of-two scales, block by block.
+struct Kept {
+    uint8_t *qg, *qu, *qx;
+    float *sg, *su, *sx;
+    long long ldn, ldk;
+    size_t bytes;
+    Kept(void* base, int m, int n, int k, bool with_x) {
+        ldn = (n + 15) / 16 * 16;
+        ldk = (k + 15) / 16 * 16;
+        const size_t codes = static_cast<size_t>(m) * ldn, codes_x = with_x ? static_cast<size_t>(m) * ldk : 0;
+        const size_t scales = static_cast<size_t>(m) * ((n + kFp8Block - 1) / kFp8Block);
+        const size_t scales_x = with_x ? static_cast<size_t>(m) * ((k + kFp8Block - 1) / kFp8Block) : 0;
+        qg = static_cast<uint8_t*>(base);
+        qu = qg + codes;
+        qx = qu + codes;
+        sg = reinterpret_cast<float*>(qx + codes_x);
+        su = sg + scales;
+        sx = su + scales;
+        bytes = 2 * codes + codes_x + 4 * (2 * scales + scales_x);
+    }
+};
 
 // One quantised operand: codes, row pitch, scales and their strides.
 struct Fp8Matrix {
@@ -329,12 +364,7 @@ int b200_fp8_dequantize_rows(const void* q, int64_t ldq, const float* sf, int64_
     if ((rc = check_matrix(what, "q", q, ldq, k, 1))) return rc;
     DenseCall call(device, stream);
     if (call.rc) return call.rc;
-    const long long blocks = (static_cast<long long>(rows) * ((k + 7) / 8) + 255) / 256;
-    if (blocks > 0x7FFFFFFFll) return fail(B200_E_LIMIT, "%s: rows=%d and k=%d are too many for one launch", what, rows, k);
-    auto* kernel = out_dtype == B200_DTYPE_BF16 ? &fp8_dequantize_rows<true> : &fp8_dequantize_rows<false>;
-    return launch_dense("fp8_dequantize_rows", kernel, dim3(static_cast<unsigned>(blocks)), 256, 0u, call.stream,
-                        static_cast<const uint8_t*>(q), static_cast<long long>(ldq), sf, static_cast<long long>(sf_row),
-                        static_cast<long long>(sf_col), rows, k, static_cast<uint16_t*>(out), static_cast<long long>(ldo));
+    return dequantize_rows_launch(what, q, ldq, sf, sf_row, sf_col, rows, k, out_dtype, out, ldo, call);
 }
 
 int b200_fp8_gemm(const void* a, int64_t lda, const float* sfa, int64_t sfa_row, int64_t sfa_col, const void* b, int64_t ldb,
@@ -356,7 +386,7 @@ int b200_fp8_gemm(const void* a, int64_t lda, const float* sfa, int64_t sfa_row,
 }
 
 size_t b200_fp8_linear_scratch_bytes(int m, int k) {
-    if (m <= 0 || k <= 0) return 0;
+    if (m <= kFuseMost || k <= 0) return 0;          // quantised on the way into the product
     return fp8_codes_bytes(m, k) + static_cast<size_t>(m) * ((k + kFp8Block - 1) / kFp8Block) * 4;
 }
 
@@ -372,10 +402,30 @@ int b200_fp8_linear(const void* x, int64_t ldx, int dtype, const void* w, int64_
     if (ldx < k) return fail(B200_E_ALIGN, "%s: ldx=%lld must be at least k=%d", what, (long long)ldx, k);
     if ((rc = check_matrix(what, "w", w, ldw, k, 1))) return rc;
     if ((rc = check_matrix(what, "y", y, ldy, n, 2))) return rc;
-    if (!scratch || !aligned16(scratch) || scratch_bytes < b200_fp8_linear_scratch_bytes(m, k))
+    if (m > kFuseMost && (!scratch || !aligned16(scratch) || scratch_bytes < b200_fp8_linear_scratch_bytes(m, k)))
         return fail(B200_E_WORKSPACE, "%s: needs %zu scratch bytes, 16-byte aligned", what, b200_fp8_linear_scratch_bytes(m, k));
     DenseCall call(device, stream);
     if (call.rc) return call.rc;
+    if (m <= kFuseMost) {
+        FewProblem p;
+        memset(&p, 0, sizeof p);
+        if ((rc = encode_matrix_map(&p.w[0], w, 1, k, n, ldw, 128, 128))) return rc;
+        p.x16 = static_cast<const uint16_t*>(x);
+        p.ldx = ldx;
+        p.k = k;
+        p.vec = aligned16(x) && ldx % 8 == 0;
+        p.sfb = sfw;
+        p.sfb_row = sfw_row;
+        p.sfb_col = sfw_col;
+        p.c = static_cast<uint16_t*>(y);
+        p.ldc = ldy;
+        p.m = m;
+        p.n = n;
+        p.steps = (k + kFp8Block - 1) / kFp8Block;
+        p.status = status ? status : call.st->status;
+        return dtype == B200_DTYPE_BF16 ? launch_few_as<FewOp::Few8, 16, true, true>(p, call)
+                                        : launch_few_as<FewOp::Few8, 16, false, true>(p, call);
+    }
     uint8_t* q = static_cast<uint8_t*>(scratch);
     float* sf = reinterpret_cast<float*>(q + fp8_codes_bytes(m, k));
     const int64_t ldq = (k + 15) / 16 * 16;
@@ -384,9 +434,19 @@ int b200_fp8_linear(const void* x, int64_t ldx, int dtype, const void* w, int64_
     return fp8_gemm_launch(ma, mb, y, ldy, dtype, m, n, k, true, call, status);
 }
 
+size_t b200_gated_kept_bytes(int m, int n, int k, int keep_x) {
+    if (m <= 0 || n <= 0 || k <= 0) return 0;
+    return Kept(nullptr, m, n, k, keep_x != 0).bytes;
+}
+
+size_t b200_gated_backward_scratch_bytes(int m, int n, int k, int kept) {
+    if (m <= 0 || n <= 0 || k <= 0) return 0;
+    return static_cast<size_t>(m) * n * 4 + (kept ? static_cast<size_t>(m) * k * 2 : 0);
+}
+
 int b200_gated_forward(const void* x, int64_t ldx, const void* w1, int64_t ldw1, const void* w2, int64_t ldw2, int dtype, int act,
-                       void* h, int64_t ldh, void* qg, void* qu, int64_t ldq, float* sg, float* su, int64_t sf_row,
-                       int64_t sf_col, int m, int n, int k, void* stream, int device, uint32_t* status) {
+                       void* h, int64_t ldh, void* kept, size_t kept_bytes, int keep_x, int m, int n, int k, void* stream,
+                       int device, uint32_t* status) {
     const char* what = "gated forward";
     int rc;
     if ((rc = check_gated(what, dtype, act, m, n, k))) return rc;
@@ -394,15 +454,11 @@ int b200_gated_forward(const void* x, int64_t ldx, const void* w1, int64_t ldw1,
     if ((rc = check_matrix(what, "w1", w1, ldw1, k, 2))) return rc;
     if ((rc = check_matrix(what, "w2", w2, ldw2, k, 2))) return rc;
     if ((rc = check_matrix(what, "h", h, ldh, n, 2))) return rc;
-    const bool keep = qg != nullptr;
-    if (keep) {
-        if (!sg || !su) return fail(B200_E_NULL, "%s: 8-bit copies need their scales", what);
-        if ((rc = check_matrix(what, "qg", qg, ldq, n, 1))) return rc;
-        if ((rc = check_matrix(what, "qu", qu, ldq, n, 1))) return rc;
-    }
+    if (kept && (!aligned16(kept) || kept_bytes < b200_gated_kept_bytes(m, n, k, keep_x)))
+        return fail(B200_E_WORKSPACE, "%s: the 8-bit copies need %zu bytes, 16-byte aligned", what, b200_gated_kept_bytes(m, n, k, keep_x));
     DenseCall call(device, stream);
     if (call.rc) return call.rc;
-    if (m <= kFewMost && !keep) {
+    if (!kept && m <= kFewMost) {
         FewProblem f;
         memset(&f, 0, sizeof f);
         if ((rc = encode_matrix_map(&f.w[0], w1, 2, k, n, ldw1, 64, 128))) return rc;
@@ -420,123 +476,109 @@ int b200_gated_forward(const void* x, int64_t ldx, const void* w1, int64_t ldw1,
     memset(&p, 0, sizeof p);
     if ((rc = ff_projections(p, x, ldx, w1, ldw1, w2, ldw2, act, m, n, k))) return rc;
     if ((rc = encode_matrix_map(&p.out[0], h, 2, n, m, ldh, 64, 32))) return rc;
-    if (keep) {
-        if ((rc = encode_matrix_map(&p.kept[0], qg, 1, n, m, ldq, 128, 32))) return rc;
-        if ((rc = encode_matrix_map(&p.kept[1], qu, 1, n, m, ldq, 128, 32))) return rc;
-        p.sf[0] = sg;
-        p.sf[1] = su;
-        p.sf_row = sf_row;
-        p.sf_col = sf_col;
+    if (kept) {
+        const Kept v(kept, m, n, k, keep_x != 0);
+        if ((rc = encode_matrix_map(&p.kept[0], v.qg, 1, n, m, v.ldn, 128, 32))) return rc;
+        if ((rc = encode_matrix_map(&p.kept[1], v.qu, 1, n, m, v.ldn, 128, 32))) return rc;
+        p.sf[0] = v.sg;
+        p.sf[1] = v.su;
+        p.sf_row = 1;
+        p.sf_col = m;
         p.keep = 1;
+        if (keep_x && (rc = quantize_rows_launch(what, x, dtype, m, k, ldx, v.qx, v.ldk, v.sx, 1, m, 1, call))) return rc;
     }
     return launch_ff<FfMode::Forward>("ff_gemm_pair<Forward>", p, dtype, call, status);
 }
 
-int b200_gated_grad_hidden(const void* x, int64_t ldx, const void* w1, int64_t ldw1, const void* w2, int64_t ldw2, int dtype,
-                           int act, const void* dh, int64_t ld_dh, void* dg, void* du, int64_t ld_out, int m, int n, int k,
-                           void* stream, int device, uint32_t* status) {
-    const char* what = "gated grad hidden";
+int b200_gated_backward(const void* x, int64_t ldx, const void* kept, size_t kept_bytes, int keep_x, const void* w1, int64_t ldw1,
+                        const void* w2, int64_t ldw2, int dtype, int act, const void* dh, int64_t ld_dh, void* dx, int64_t ld_dx,
+                        void* dw1, void* dw2, int64_t ld_dw, int m, int n, int k, void* scratch, size_t scratch_bytes,
+                        void* stream, int device, uint32_t* status) {
+    const char* what = "gated backward";
     int rc;
+    const bool weights = dw1 || dw2;
     if ((rc = check_gated(what, dtype, act, m, n, k))) return rc;
-    if ((rc = check_matrix(what, "x", x, ldx, k, 2))) return rc;
+    if (!dx && !weights) return fail(B200_E_NULL, "%s: no gradient is asked for", what);
+    if (!kept && (rc = check_matrix(what, "x", x, ldx, k, 2))) return rc;
     if ((rc = check_matrix(what, "w1", w1, ldw1, k, 2))) return rc;
     if ((rc = check_matrix(what, "w2", w2, ldw2, k, 2))) return rc;
     if ((rc = check_matrix(what, "dh", dh, ld_dh, n, 2))) return rc;
-    if ((rc = check_matrix(what, "dg", dg, ld_out, n, 2))) return rc;
-    if ((rc = check_matrix(what, "du", du, ld_out, n, 2))) return rc;
+    if (dx && (rc = check_matrix(what, "dx", dx, ld_dx, k, 2))) return rc;
+    if (dw1 && (rc = check_matrix(what, "dw1", dw1, ld_dw, k, 2))) return rc;
+    if (dw2 && (rc = check_matrix(what, "dw2", dw2, ld_dw, k, 2))) return rc;
+    if (kept && (!aligned16(kept) || kept_bytes < b200_gated_kept_bytes(m, n, k, keep_x)))
+        return fail(B200_E_WORKSPACE, "%s: the 8-bit copies are %zu bytes, 16-byte aligned", what, b200_gated_kept_bytes(m, n, k, keep_x));
+    if (kept && weights && !keep_x) return fail(B200_E_VARIANT, "%s: the weights' gradients need an 8-bit copy of x (keep_x)", what);
+    const size_t need = b200_gated_backward_scratch_bytes(m, n, k, kept != nullptr);
+    if (!scratch || !aligned16(scratch) || scratch_bytes < need)
+        return fail(B200_E_WORKSPACE, "%s: needs %zu scratch bytes, 16-byte aligned", what, need);
     DenseCall call(device, stream);
     if (call.rc) return call.rc;
-    FfProblem p;
-    memset(&p, 0, sizeof p);
-    if ((rc = ff_projections(p, x, ldx, w1, ldw1, w2, ldw2, act, m, n, k))) return rc;
-    if ((rc = encode_matrix_map(&p.out[0], dg, 2, n, m, ld_out, 64, 32))) return rc;
-    if ((rc = encode_matrix_map(&p.out[1], du, 2, n, m, ld_out, 64, 32))) return rc;
-    p.dh = static_cast<const uint16_t*>(dh);
-    p.ld_dh = ld_dh;
-    return launch_ff<FfMode::GradHidden>("ff_gemm_pair<GradHidden>", p, dtype, call, status);
-}
-
-int b200_gated_grad_hidden_kept(const void* qg, const void* qu, int64_t ldq, const float* sg, const float* su, int64_t sf_row,
-                                int64_t sf_col, int dtype, int act, const void* dh, int64_t ld_dh, void* dg, void* du,
-                                int64_t ld_out, int m, int n, void* stream, int device) {
-    const char* what = "gated grad hidden (kept)";
-    int rc;
-    if ((rc = check_gated(what, dtype, act, m, n, 8))) return rc;
-    if (!sg || !su) return fail(B200_E_NULL, "%s: NULL scale pointer", what);
-    if ((rc = check_matrix(what, "qg", qg, ldq, n, 1))) return rc;
-    if ((rc = check_matrix(what, "qu", qu, ldq, n, 1))) return rc;
-    if ((rc = check_matrix(what, "dh", dh, ld_dh, n, 2))) return rc;
-    if ((rc = check_matrix(what, "dg", dg, ld_out, n, 2))) return rc;
-    if ((rc = check_matrix(what, "du", du, ld_out, n, 2))) return rc;
-    DenseCall call(device, stream);
-    if (call.rc) return call.rc;
-    const long long blocks = (static_cast<long long>(m) * (n / 8) + 256 * kKeptUnits - 1) / (256 * kKeptUnits);
-    if (blocks > 0x7FFFFFFFll) return fail(B200_E_LIMIT, "%s: m=%d and n=%d are too many for one launch", what, m, n);
-    auto* kernel = dtype == B200_DTYPE_BF16 ? &gated_grad_kept<true> : &gated_grad_kept<false>;
-    return launch_dense("gated_grad_kept", kernel, dim3(static_cast<unsigned>(blocks)), 256, 0u, call.stream,
-                        static_cast<const uint8_t*>(qg), static_cast<const uint8_t*>(qu), static_cast<long long>(ldq), sg, su,
-                        static_cast<long long>(sf_row), static_cast<long long>(sf_col), static_cast<const uint16_t*>(dh),
-                        static_cast<long long>(ld_dh), static_cast<uint16_t*>(dg), static_cast<uint16_t*>(du),
-                        static_cast<long long>(ld_out), m, n, act == B200_ACT_GELU ? 1 : 0);
-}
-
-int b200_gated_grad_input(const void* dg, const void* du, int64_t ld_g, const void* w1, int64_t ldw1, const void* w2,
-                          int64_t ldw2, int dtype, void* dx, int64_t ld_dx, int m, int n, int k, void* stream, int device,
-                          uint32_t* status) {
-    const char* what = "gated grad input";
-    int rc;
-    if ((rc = check_gated(what, dtype, B200_ACT_SILU, m, n, k))) return rc;
-    if ((rc = check_matrix(what, "dg", dg, ld_g, n, 2))) return rc;
-    if ((rc = check_matrix(what, "du", du, ld_g, n, 2))) return rc;
-    if ((rc = check_matrix(what, "w1", w1, ldw1, k, 2))) return rc;
-    if ((rc = check_matrix(what, "w2", w2, ldw2, k, 2))) return rc;
-    if ((rc = check_matrix(what, "dx", dx, ld_dx, k, 2))) return rc;
-    DenseCall call(device, stream);
-    if (call.rc) return call.rc;
-    FfProblem p;
-    memset(&p, 0, sizeof p);
-    if ((rc = encode_matrix_map(&p.a[0], dg, 2, n, m, ld_g, 64, 128))) return rc;
-    if ((rc = encode_matrix_map(&p.a[1], du, 2, n, m, ld_g, 64, 128))) return rc;
-    if ((rc = encode_matrix_map(&p.b[0], w1, 2, k, n, ldw1, 64, 64))) return rc;
-    if ((rc = encode_matrix_map(&p.b[1], w2, 2, k, n, ldw2, 64, 64))) return rc;
-    if ((rc = encode_matrix_map(&p.out[0], dx, 2, k, m, ld_dx, 64, 32))) return rc;
-    p.rows = m;
-    p.cols = k;
-    p.k_tiles = (n + 63) / 64;
-    p.segments = 2;
-    p.m_tiles = (m + 255) / 256;
-    p.n_tiles = (k + 255) / 256;
-    p.batches = 1;
-    return launch_ff<FfMode::GradInput>("ff_gemm_pair<GradInput>", p, dtype, call, status);
-}
-
-int b200_gated_grad_weight(const void* dg, const void* du, int64_t ld_g, const void* x, int64_t ldx, int dtype, void* dw1,
-                           void* dw2, int64_t ld_dw, int m, int n, int k, void* stream, int device, uint32_t* status) {
-    const char* what = "gated grad weight";
-    int rc;
-    if ((rc = check_gated(what, dtype, B200_ACT_SILU, m, n, k))) return rc;
-    if ((rc = check_matrix(what, "dg", dg, ld_g, n, 2))) return rc;
-    if ((rc = check_matrix(what, "du", du, ld_g, n, 2))) return rc;
-    if ((rc = check_matrix(what, "x", x, ldx, k, 2))) return rc;
-    if ((rc = check_matrix(what, "dw1", dw1, ld_dw, k, 2))) return rc;
-    if ((rc = check_matrix(what, "dw2", dw2, ld_dw, k, 2))) return rc;
-    DenseCall call(device, stream);
-    if (call.rc) return call.rc;
-    FfProblem p;
-    memset(&p, 0, sizeof p);
-    if ((rc = encode_matrix_map(&p.a[0], dg, 2, n, m, ld_g, 64, 64))) return rc;
-    if ((rc = encode_matrix_map(&p.a[1], du, 2, n, m, ld_g, 64, 64))) return rc;
-    if ((rc = encode_matrix_map(&p.b[0], x, 2, k, m, ldx, 64, 64))) return rc;
-    if ((rc = encode_matrix_map(&p.out[0], dw1, 2, k, n, ld_dw, 64, 32))) return rc;
-    if ((rc = encode_matrix_map(&p.out[1], dw2, 2, k, n, ld_dw, 64, 32))) return rc;
-    p.rows = n;
-    p.cols = k;
-    p.k_tiles = (m + 63) / 64;
-    p.segments = 1;
-    p.m_tiles = (n + 255) / 256;
-    p.n_tiles = (k + 255) / 256;
-    p.batches = 2;
-    return launch_ff<FfMode::GradWeight>("ff_gemm_pair<GradWeight>", p, dtype, call, status);
+    uint16_t* dg = static_cast<uint16_t*>(scratch);
+    uint16_t* du = dg + static_cast<size_t>(m) * n;
+    // the gradients of the two projections
+    if (kept) {
+        const Kept v(const_cast<void*>(kept), m, n, k, keep_x != 0);
+        const unsigned row_groups = static_cast<unsigned>((m + kKeptRows - 1) / kKeptRows);
+        const dim3 grid((n + kKeptCols - 1) / kKeptCols, row_groups < 65535u ? row_groups : 65535u);
+        auto* kernel = dtype == B200_DTYPE_BF16 ? &gated_grad_kept<true> : &gated_grad_kept<false>;
+        if ((rc = launch_dense("gated_grad_kept", kernel, grid, kKeptThreads, 0u, call.stream, (const uint8_t*)v.qg, (const uint8_t*)v.qu,
+                               v.ldn, (const float*)v.sg, (const float*)v.su, 1ll, (long long)m, static_cast<const uint16_t*>(dh),
+                               static_cast<long long>(ld_dh), dg, du, (long long)n, m, n, act == B200_ACT_GELU ? 1 : 0))) return rc;
+        if (weights) {      // x back to 16 bits, exactly: an operand of the weights' gradients
+            uint16_t* x16 = du + static_cast<size_t>(m) * n;
+            if ((rc = dequantize_rows_launch(what, v.qx, v.ldk, v.sx, 1, m, m, k, dtype, x16, k, call))) return rc;
+            x = x16;
+            ldx = k;
+        }
+    } else {
+        FfProblem p;
+        memset(&p, 0, sizeof p);
+        if ((rc = ff_projections(p, x, ldx, w1, ldw1, w2, ldw2, act, m, n, k))) return rc;
+        if ((rc = encode_matrix_map(&p.out[0], dg, 2, n, m, n, 64, 32))) return rc;
+        if ((rc = encode_matrix_map(&p.out[1], du, 2, n, m, n, 64, 32))) return rc;
+        p.dh = static_cast<const uint16_t*>(dh);
+        p.ld_dh = ld_dh;
+        if ((rc = launch_ff<FfMode::GradHidden>("ff_gemm_pair<GradHidden>", p, dtype, call, status))) return rc;
+    }
+    if (dx) {
+        FfProblem p;
+        memset(&p, 0, sizeof p);
+        if ((rc = encode_matrix_map(&p.a[0], dg, 2, n, m, n, 64, 128))) return rc;
+        if ((rc = encode_matrix_map(&p.a[1], du, 2, n, m, n, 64, 128))) return rc;
+        if ((rc = encode_matrix_map(&p.b[0], w1, 2, k, n, ldw1, 64, 64))) return rc;
+        if ((rc = encode_matrix_map(&p.b[1], w2, 2, k, n, ldw2, 64, 64))) return rc;
+        if ((rc = encode_matrix_map(&p.out[0], dx, 2, k, m, ld_dx, 64, 32))) return rc;
+        p.rows = m;
+        p.cols = k;
+        p.k_tiles = (n + 63) / 64;
+        p.segments = 2;
+        p.m_tiles = (m + 255) / 256;
+        p.n_tiles = (k + 255) / 256;
+        p.batches = 1;
+        if ((rc = launch_ff<FfMode::GradInput>("ff_gemm_pair<GradInput>", p, dtype, call, status))) return rc;
+    }
+    if (weights) {
+        FfProblem p;
+        memset(&p, 0, sizeof p);
+        p.batches = 0;
+        for (int i = 0; i < 2; ++i) {      // one launch for what is asked for
+            void* out = i == 0 ? dw1 : dw2;
+            if (!out) continue;
+            if ((rc = encode_matrix_map(&p.a[p.batches], i == 0 ? dg : du, 2, n, m, n, 64, 64))) return rc;
+            if ((rc = encode_matrix_map(&p.out[p.batches], out, 2, k, n, ld_dw, 64, 32))) return rc;
+            ++p.batches;
+        }
+        if ((rc = encode_matrix_map(&p.b[0], x, 2, k, m, ldx, 64, 64))) return rc;
+        p.rows = n;
+        p.cols = k;
+        p.k_tiles = (m + 63) / 64;
+        p.segments = 1;
+        p.m_tiles = (n + 255) / 256;
+        p.n_tiles = (k + 255) / 256;
+        if ((rc = launch_ff<FfMode::GradWeight>("ff_gemm_pair<GradWeight>", p, dtype, call, status))) return rc;
+    }
+    return 0;
 }
 
 }  // extern "C"

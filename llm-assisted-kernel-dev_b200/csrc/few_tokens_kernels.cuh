@@ -8,9 +8,11 @@
 //
 //   Few8      fp8: fp32 sums of one 128-wide block in tensor memory, scaled and added up in registers (one weight
 //             row per lane, one column per token), as in fp8_gemm_pair
+//             With kFuse the tokens come as 16-bit rows and four more warps quantise them on their way into shared
+//             memory (up to 16 tokens: every tile of W repeats that work, and a launch of its own costs more)
 //   FewGated  16-bit: g and u of the same rows and tokens side by side in tensor memory, h formed after the exchange
 //
-// Seven warps: 0-3 sums and results, 4 MMA issuer, 5 weight loads, 6 token loads (and their scales).
+// Seven warps: 0-3 sums and results, 4 MMA issuer, 5 weight loads, 6 token loads (and their scales); 7-10 quantise (kFuse).
 #pragma once
 
 #include "dense_tiles.cuh"
@@ -22,6 +24,9 @@ enum class FewOp { Few8, FewGated };
 
 struct FewProblem {
     CUtensorMap w[2], x;
+    const uint16_t* x16;         // kFuse: the tokens
+    long long ldx;
+    int k, vec;                  // vec: rows of x start on 16-byte boundaries
     const float* sfa;            // Few8: token scales, [token * sfa_row + block * sfa_col]
     const float* sfb;            // Few8: weight scales, [(row / 128) * sfb_row + block * sfb_col]
     long long sfa_row, sfa_col, sfb_row, sfb_col;
@@ -59,7 +64,8 @@ template <FewOp kOp, int kTokens> constexpr uint32_t few_smem_bytes() {
     using S = FewShape<kOp, kTokens>;
     return 1024u + S::kStages * S::kStageBytes + sizeof(FewControl<kOp, kTokens>);
 }
-constexpr int kFewThreads = 224;
+constexpr int kFewThreads = 224, kFewFuseThreads = 352;
+constexpr int kFuseAhead = 4;            // blocks of k whose tokens a quantising half-warp loads at a time
 
 __device__ __forceinline__ float4 ld_cluster_v4f(uint32_t cluster_addr) {
     float4 v;
@@ -83,8 +89,8 @@ template <int kN> __device__ __forceinline__ void tc_ld_cols(uint32_t taddr, uin
     else tc_ld_x32(taddr, v);
 }
 
-template <FewOp kOp, int kTokens, bool kBf16>
-__global__ void __launch_bounds__(kFewThreads, FewShape<kOp, kTokens>::kCtasPerSm)
+template <FewOp kOp, int kTokens, bool kBf16, bool kFuse = false>
+__global__ void __launch_bounds__(kFuse ? kFewFuseThreads : kFewThreads, FewShape<kOp, kTokens>::kCtasPerSm)
 few_tokens_gemm(const __grid_constant__ FewProblem p) {
     using S = FewShape<kOp, kTokens>;
     constexpr bool kFp8 = S::kFp8;
@@ -105,7 +111,7 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(smem_u32(&ctl->wfull[s]), 1);
-            mbar_init(smem_u32(&ctl->tfull[s]), 1);
+            mbar_init(smem_u32(&ctl->tfull[s]), kFuse ? 4 : 1);       // kFuse: the quantising warps
             mbar_init(smem_u32(&ctl->empty[s]), 1);
             mbar_init(smem_u32(&ctl->sfull[s]), 32);
             mbar_init(smem_u32(&ctl->sempty[s]), 4);
@@ -131,7 +137,57 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
 
     float sum[kFp8 ? kTokens : 1];      // Few8: this lane's weight row, all tokens
     bool ok = true;
-    if (warp == 5 || warp == 6) {
+    if (kFuse && (warp == 6 || warp >= 7)) {
+        // ------------------------------ tokens: quantised here (a half-warp holds one token's block of 128)
+        if (warp >= 7) {
+            const int half = (warp - 7) * 2 + (lane >> 4), l = lane & 15;
+            uint32_t s = 0, ph = 0;
+            for (int i0 = 0; ok && i0 < count; i0 += kFuseAhead) {
+                uint4 v[kFuseAhead][kTokens / 8];
+#pragma unroll
+                for (int a = 0; a < kFuseAhead; ++a)
+#pragma unroll
+                    for (int t = 0; t < kTokens / 8; ++t) {
+                        const int token = token0 + t * 8 + half, col = (begin + i0 + a) * kFp8Block + l * 8;
+                        const int valid = token < p.m && i0 + a < count ? p.k - col : 0;
+                        const uint16_t* src = p.x16 + token * p.ldx + col;
+                        v[a][t] = p.vec ? load_8x16<true>(src, valid) : load_8x16<false>(src, valid);
+                    }
+#pragma unroll
+                for (int a = 0; a < kFuseAhead; ++a) {
+                    if (i0 + a >= count) break;
+                    ok = mbar_wait_converged(smem_u32(&ctl->empty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense) &&
+                         mbar_wait_converged(smem_u32(&ctl->sempty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense);
+                    if (!ok) break;
+                    const uint32_t tile = smem_base + s * S::kStageBytes + S::kWeightBytes;
+#pragma unroll
+                    for (int t = 0; t < kTokens / 8; ++t) {
+                        const int row = t * 8 + half;       // rows past the last token stay as they are: nobody reads their sums
+                        float f[8];
+                        to_float8<kBf16>(v[a][t], f);
+                        float m = amax8(f);
+#pragma unroll
+                        for (int d = 8; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+                        const LinearScale c(fmaxf(m, kAmaxFloor));
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) f[j] = c(f[j]);
+                        if (token0 + row < p.m) {
+                            const uint32_t at = tile + row * 128 + (static_cast<uint32_t>((l >> 1) ^ (row & 7)) << 4) + (l & 1) * 8;
+                            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(pack_e4m3x4(f[0], f[1], f[2], f[3])),
+                                         "r"(pack_e4m3x4(f[4], f[5], f[6], f[7]))
+                                         : "memory");
+                            if (l == 0) ctl->scale[s][row] = c.scale;
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    mbar_arrive_elect(smem_u32(&ctl->tfull[s]));
+                    if (++s == kStages) { s = 0; ph ^= 1u; }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 5 || warp == 6) {
         // ------------------------------ loads
         uint32_t s = 0, ph = 0;
         for (int i = 0; i < count; ++i) {
@@ -172,11 +228,10 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
         constexpr uint32_t kIdesc = idesc_dense(128, kTokens, kFp8 ? 0u : (kBf16 ? 1u : 0u), false, false);
         uint32_t s = 0, ph = 0;
         for (int i = 0; i < count; ++i) {
-            ok = mbar_wait<true>(smem_u32(&ctl->wfull[s]), ph, abort_flag, p.status, kStatusDense) &&
-                 mbar_wait<true>(smem_u32(&ctl->tfull[s]), ph, abort_flag, p.status, kStatusDense);
+            ok = mbar_wait_converged(smem_u32(&ctl->wfull[s]), ph, abort_flag, p.status, kStatusDense) &&
+                 mbar_wait_converged(smem_u32(&ctl->tfull[s]), ph, abort_flag, p.status, kStatusDense);
             if (kFp8 && ok && i >= 2)
-                ok = mbar_wait<true>(smem_u32(&ctl->acc_release[i & 1]), ((i >> 1) - 1) & 1, abort_flag, p.status, kStatusDense);
-            ok = __all_sync(0xffffffffu, ok);
+                ok = mbar_wait_converged(smem_u32(&ctl->acc_release[i & 1]), ((i >> 1) - 1) & 1, abort_flag, p.status, kStatusDense);
             if (!ok) break;
             tc_fence_after_sync();
             const uint32_t w = dense_desc_lo<false>(smem_base + s * S::kStageBytes);
@@ -211,9 +266,9 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
         for (int i = 0; i < count; ++i) {
             const uint64_t b2 = pack_f32x2(__float_as_uint(b_next), __float_as_uint(b_next));
             if (i + 1 < count) b_next = sb[(i + 1) * p.sfb_col];
-            ok = mbar_wait<true>(smem_u32(&ctl->sfull[s]), ph, abort_flag, p.status, kStatusDense) &&
-                 mbar_wait<true>(smem_u32(&ctl->acc_full[i & 1]), (i >> 1) & 1, abort_flag, p.status, kStatusDense);
-            ok = __all_sync(0xffffffffu, ok);
+            // the scales came with the tokens (kFuse) or by copies of their own
+            ok = mbar_wait_converged(smem_u32(kFuse ? &ctl->tfull[s] : &ctl->sfull[s]), ph, abort_flag, p.status, kStatusDense) &&
+                 mbar_wait_converged(smem_u32(&ctl->acc_full[i & 1]), (i >> 1) & 1, abort_flag, p.status, kStatusDense);
             if (!ok) break;
             tc_fence_after_sync();
             const uint32_t scales = smem_u32(&ctl->scale[s][0]);
@@ -233,10 +288,8 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
             }
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(smem_u32(&ctl->acc_release[i & 1]));
-                mbar_arrive(smem_u32(&ctl->sempty[s]));
-            }
+            mbar_arrive_elect(smem_u32(&ctl->acc_release[i & 1]));
+            mbar_arrive_elect(smem_u32(&ctl->sempty[s]));
             if (++s == kStages) { s = 0; ph ^= 1u; }
         }
 #pragma unroll

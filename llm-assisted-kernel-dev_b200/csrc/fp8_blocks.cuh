@@ -96,29 +96,29 @@ fp8_quantize_rows(const uint16_t* __restrict__ x, long long ldx, int rows, int k
                   float* __restrict__ sf, long long sf_row, long long sf_col) {
     griddep_wait();
     griddep_launch_dependents();   // in this order: whoever starts from here on finds all work before this kernel complete
-    const int blocks_k = (k + kFp8Block - 1) / kFp8Block;
-    const long long units = static_cast<long long>(rows) * blocks_k;
+    const unsigned blocks_k = (k + kFp8Block - 1) / kFp8Block;
+    const unsigned units = static_cast<unsigned>(rows) * blocks_k;       // below 2^32 (checked on the host)
     const int half = threadIdx.x >> 4, l = threadIdx.x & 15;
-    const long long first = static_cast<long long>(blockIdx.x) * (kRowThreads / 16 * kRowUnits) + half;
+    const unsigned first = blockIdx.x * (kRowThreads / 16 * kRowUnits) + half;
     uint4 v[kRowUnits];
+    unsigned row[kRowUnits], blk[kRowUnits];
 #pragma unroll
     for (int i = 0; i < kRowUnits; ++i) {
-        const long long u = first + i * (kRowThreads / 16);
-        const long long r = u / blocks_k;
-        const int col = static_cast<int>(u - r * blocks_k) * kFp8Block + l * 8;
-        v[i] = load_8x16<kVec>(x + r * ldx + col, u < units ? k - col : 0);
+        const unsigned u = first + i * (kRowThreads / 16);
+        row[i] = u / blocks_k;
+        blk[i] = u - row[i] * blocks_k;
+        const int col = blk[i] * kFp8Block + l * 8;
+        v[i] = load_8x16<kVec>(x + row[i] * ldx + col, u < units ? k - col : 0);
     }
 #pragma unroll
     for (int i = 0; i < kRowUnits; ++i) {
-        const long long u = first + i * (kRowThreads / 16);
-        const long long r = u / blocks_k;
-        const int b = static_cast<int>(u - r * blocks_k), col = b * kFp8Block + l * 8;
+        const int col = blk[i] * kFp8Block + l * 8;
         float f[8];
         to_float8<kBf16>(v[i], f);
         float m = amax8(f);
 #pragma unroll
         for (int s = 8; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-        if (u >= units) continue;
+        if (first + i * (kRowThreads / 16) >= units) continue;
         m = fmaxf(m, kAmaxFloor);
         float scale;
         if constexpr (kPow2) {
@@ -132,8 +132,8 @@ fp8_quantize_rows(const uint16_t* __restrict__ x, long long ldx, int rows, int k
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] = c(f[j]);
         }
-        store_codes(q + r * ldq + col, f, k - col);
-        if (l == 0) sf[r * sf_row + b * sf_col] = scale;
+        store_codes(q + row[i] * ldq + col, f, k - col);
+        if (l == 0) sf[row[i] * sf_row + blk[i] * sf_col] = scale;
     }
 }
 
@@ -186,11 +186,11 @@ fp8_dequantize_rows(const uint8_t* __restrict__ q, long long ldq, const float* _
                     long long sf_col, int rows, int k, uint16_t* __restrict__ out, long long ldo) {
     griddep_launch_dependents();
     griddep_wait();
-    const int per_row = (k + 7) / 8;
-    const long long u = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-    if (u >= static_cast<long long>(rows) * per_row) return;
-    const long long r = u / per_row;
-    const int col = static_cast<int>(u - r * per_row) * 8;
+    const unsigned per_row = (k + 7) / 8;
+    const unsigned u = blockIdx.x * 256u + threadIdx.x;                 // rows * per_row < 2^32 (checked on the host)
+    const unsigned r = u / per_row;
+    if (r >= static_cast<unsigned>(rows)) return;
+    const int col = (u - r * per_row) * 8;
     const float s = sf[r * sf_row + (col / kFp8Block) * sf_col];
     const int valid = k - col;
     const uint8_t* src = q + r * ldq + col;

@@ -347,53 +347,63 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
 }
 
 // dg and du from the 8-bit copies of g and u: a streaming pass, 2 bytes of codes, 2 of dh and 4 of results per
-// element.  Eight columns per thread, kKeptUnits groups loaded before the first is used.
-constexpr int kKeptUnits = 2;
+// element.  A thread takes 16 columns of kKeptRows rows, all loaded before the first is used.
+__device__ __forceinline__ uint4 load_codes16(const uint8_t* p, bool all) {
+    if (all) return *reinterpret_cast<const uint4*>(p);
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    return make_uint4(v.x, v.y, 0, 0);
+}
+constexpr int kKeptRows = 2, kKeptThreads = 128;
+constexpr int kKeptCols = kKeptThreads * 16;
 template <bool kBf16>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kKeptThreads)
 gated_grad_kept(const uint8_t* __restrict__ qg, const uint8_t* __restrict__ qu, long long ldq, const float* __restrict__ sg,
                 const float* __restrict__ su, long long sf_row, long long sf_col, const uint16_t* __restrict__ dh,
                 long long ld_dh, uint16_t* __restrict__ dg, uint16_t* __restrict__ du, long long ld_out, int rows, int n,
                 int gelu) {
     griddep_launch_dependents();
     griddep_wait();
-    const int per_row = n / 8;
-    const long long units = static_cast<long long>(rows) * per_row;
-    const long long first = static_cast<long long>(blockIdx.x) * (256 * kKeptUnits) + threadIdx.x;
-    uint2 a[kKeptUnits], b[kKeptUnits];
-    uint4 d[kKeptUnits];
-    float s1[kKeptUnits], s2[kKeptUnits];
+    const int col = blockIdx.x * kKeptCols + threadIdx.x * 16;
+    if (col >= n) return;
+    const bool upper = col + 8 < n;              // n is a multiple of 8: the thread's second half may be missing
+    for (long long r0 = static_cast<long long>(blockIdx.y) * kKeptRows; r0 < rows; r0 += static_cast<long long>(gridDim.y) * kKeptRows) {
+        uint4 a[kKeptRows], b[kKeptRows], d[kKeptRows][2];
+        float s1[kKeptRows], s2[kKeptRows];
 #pragma unroll
-    for (int i = 0; i < kKeptUnits; ++i) {
-        const long long u = first + i * 256;
-        if (u >= units) break;
-        const long long r = u / per_row;
-        const int col = static_cast<int>(u - r * per_row) * 8;
-        a[i] = *reinterpret_cast<const uint2*>(qg + r * ldq + col);
-        b[i] = *reinterpret_cast<const uint2*>(qu + r * ldq + col);
-        d[i] = *reinterpret_cast<const uint4*>(dh + r * ld_dh + col);
-        s1[i] = sg[r * sf_row + (col / kFp8Block) * sf_col];
-        s2[i] = su[r * sf_row + (col / kFp8Block) * sf_col];
-    }
-#pragma unroll
-    for (int i = 0; i < kKeptUnits; ++i) {
-        const long long u = first + i * 256;
-        if (u >= units) break;
-        const long long r = u / per_row;
-        const int col = static_cast<int>(u - r * per_row) * 8;
-        float e[8];
-        to_float8<kBf16>(d[i], e);
-        uint32_t og[4], ou[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 g = unpack_e4m3x2((j < 2 ? a[i].x : a[i].y) >> (16 * (j & 1)));
-            const float2 v = unpack_e4m3x2((j < 2 ? b[i].x : b[i].y) >> (16 * (j & 1)));
-            const GateValue g0 = gate<true>(g.x * s1[i], gelu), g1 = gate<true>(g.y * s1[i], gelu);
-            og[j] = pack_16<kBf16>(e[2 * j] * (v.x * s2[i]) * g0.slope, e[2 * j + 1] * (v.y * s2[i]) * g1.slope);
-            ou[j] = pack_16<kBf16>(e[2 * j] * g0.value, e[2 * j + 1] * g1.value);
+        for (int i = 0; i < kKeptRows; ++i) {
+            const long long r = r0 + i;
+            if (r >= rows) break;
+            a[i] = load_codes16(qg + r * ldq + col, upper);
+            b[i] = load_codes16(qu + r * ldq + col, upper);
+            const uint4* dr = reinterpret_cast<const uint4*>(dh + r * ld_dh + col);
+            d[i][0] = dr[0];
+            d[i][1] = upper ? dr[1] : make_uint4(0, 0, 0, 0);
+            s1[i] = sg[r * sf_row + (col / kFp8Block) * sf_col];
+            s2[i] = su[r * sf_row + (col / kFp8Block) * sf_col];
         }
-        *reinterpret_cast<uint4*>(dg + r * ld_out + col) = make_uint4(og[0], og[1], og[2], og[3]);
-        *reinterpret_cast<uint4*>(du + r * ld_out + col) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+#pragma unroll
+        for (int i = 0; i < kKeptRows; ++i) {
+            const long long r = r0 + i;
+            if (r >= rows) break;
+            const uint32_t wa[4] = {a[i].x, a[i].y, a[i].z, a[i].w}, wb[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+                if (part == 1 && !upper) break;
+                float e[8];
+                to_float8<kBf16>(d[i][part], e);
+                uint32_t og[4], ou[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 g = unpack_e4m3x2(wa[part * 2 + j / 2] >> (16 * (j & 1)));
+                    const float2 v = unpack_e4m3x2(wb[part * 2 + j / 2] >> (16 * (j & 1)));
+                    const GateValue g0 = gate<true>(g.x * s1[i], gelu), g1 = gate<true>(g.y * s1[i], gelu);
+                    og[j] = pack_16<kBf16>(e[2 * j] * (v.x * s2[i]) * g0.slope, e[2 * j + 1] * (v.y * s2[i]) * g1.slope);
+                    ou[j] = pack_16<kBf16>(e[2 * j] * g0.value, e[2 * j + 1] * g1.value);
+                }
+                *reinterpret_cast<uint4*>(dg + r * ld_out + col + part * 8) = make_uint4(og[0], og[1], og[2], og[3]);
+                *reinterpret_cast<uint4*>(du + r * ld_out + col + part * 8) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+            }
+        }
     }
 }
 

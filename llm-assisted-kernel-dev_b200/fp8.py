@@ -182,11 +182,12 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_sf: torch.Tensor, *
         if out.dtype != x.dtype:
             raise ValueError(f"fp8_linear: out must be {x.dtype}, got {out.dtype}")
     if m:
-        nbytes = m * _padded(k, 16) + 4 * m * -(-k // BLOCK)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        # up to 16 rows are quantised inside the product's kernel
+        nbytes = m * _padded(k, 16) + 4 * m * -(-k // BLOCK) if m > 16 else 0
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         code = _lib.load().b200_fp8_linear(x2.data_ptr(), _row_pitch(x2), dtype, weight.data_ptr(), _row_pitch(weight),
                                            weight_sf.data_ptr(), weight_sf.stride(0), weight_sf.stride(1), y.data_ptr(),
-                                           _row_pitch(y), m, n, k, scratch.data_ptr(), nbytes, _raw_stream(device.index),
+                                           _row_pitch(y), m, n, k, scratch.data_ptr() if nbytes else None, nbytes, _raw_stream(device.index),
                                            device.index, None)
         if code:
             _lib.check(code)

@@ -42,29 +42,46 @@ def _check(x, w1, w2, activation, keep="inputs"):
             raise ValueError("x, w1 and w2 must have one type and live on one device")
 
 
-def _stream(t: torch.Tensor):
-    index = t.device.index
-    return fp8._raw_stream(index), index
+def _kept_bytes(m: int, n: int, k: int, keep_x: bool) -> int:
+    rows = 2 * fp8._padded(n, 16) + 4 * 2 * -(-n // fp8.BLOCK)
+    if keep_x:
+        rows += fp8._padded(k, 16) + 4 * -(-k // fp8.BLOCK)
+    return m * rows
 
 
-def _mat(t: torch.Tensor):
-    return t.data_ptr(), fp8._row_pitch(t)
+def kept_copies(kept: torch.Tensor, m: int, n: int, k: int):
+    """``(g, g_sf, u, u_sf, x, x_sf)``: the quantised matrices inside the buffer that ``keep="fp8"`` saves (``x`` and
+    ``x_sf`` None if the weights need no gradient), in the form ``fp8.dequantize_fp8`` takes."""
+    keep_x = kept.numel() != _kept_bytes(m, n, k, False)
+    widths = (n, n, k) if keep_x else (n, n)
+    codes, scales, at = [], [], 0
+    for w in widths:
+        pitch = fp8._padded(w, 16)
+        codes.append(kept[at:at + m * pitch].view(m, pitch)[:, :w].view(fp8.E4M3))
+        at += m * pitch
+    for w in widths:
+        blocks = -(-w // fp8.BLOCK)
+        scales.append(kept[at:at + 4 * m * blocks].view(torch.float32).view(blocks, m).t())
+        at += 4 * m * blocks
+    out = [t for pair in zip(codes, scales) for t in pair]
+    return tuple(out) if keep_x else (*out, None, None)
 
 
-def _forward(x, w1, w2, act: int, kept):
-    """h of matrices; ``kept`` None or (qg, sg, qu, su) to be filled."""
+def _forward(x, w1, w2, act: int, kept, keep_x: bool):
+    """h of matrices; ``kept`` None or the buffer to be filled."""
     m, k = x.shape
     n = w1.shape[0]
-    h = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    device = x.device
+    h = torch.empty((m, n), dtype=x.dtype, device=device)
     if m == 0:
         return h
-    if kept is None:
-        tail = (None, None, 0, None, None, 0, 0)
-    else:
-        qg, sg, qu, su = kept
-        tail = (qg.data_ptr(), qu.data_ptr(), fp8._row_pitch(qg), sg.data_ptr(), su.data_ptr(), sg.stride(0), sg.stride(1))
-    _lib.check(_lib.load().b200_gated_forward(*_mat(x), *_mat(w1), *_mat(w2), fp8._dtype_code(x.dtype, "x"), act, h.data_ptr(), n,
-                                              *tail, m, n, k, *_stream(x), None))
+    pitch = fp8._row_pitch
+    code = _lib.load().b200_gated_forward(x.data_ptr(), pitch(x), w1.data_ptr(), pitch(w1), w2.data_ptr(), pitch(w2),
+                                          fp8._DTYPES[x.dtype], act, h.data_ptr(), n, None if kept is None else kept.data_ptr(),
+                                          0 if kept is None else kept.numel(), keep_x, m, n, k, fp8._raw_stream(device.index),
+                                          device.index, None)
+    if code:
+        _lib.check(code)
     return h
 
 
@@ -73,51 +90,44 @@ class _GatedFfn(torch.autograd.Function):
     def forward(ctx, x, w1, w2, act, keep):
         ctx.act, ctx.keep = act, keep
         if keep == "inputs":
-            ctx.save_for_backward(x, w1, w2)
-            return _forward(x, w1, w2, act, None)
-        kept = (*fp8.empty_rows(x.shape[0], w1.shape[0], x.device), *fp8.empty_rows(x.shape[0], w1.shape[0], x.device))
-        h = _forward(x, w1, w2, act, kept)
-        qx, sx = fp8.quantize_fp8(x, pow2=True) if ctx.needs_input_grad[1] or ctx.needs_input_grad[2] else (None, None)
-        ctx.save_for_backward(w1, w2, *kept, qx, sx)
-        return h
+            ctx.save_for_backward(w1, w2, x)
+            return _forward(x, w1, w2, act, None, False)
+        m, k = x.shape
+        keep_x = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        kept = torch.empty(_kept_bytes(m, w1.shape[0], k, keep_x), dtype=torch.uint8, device=x.device)
+        ctx.save_for_backward(w1, w2, kept)
+        return _forward(x, w1, w2, act, kept, keep_x)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
-        lib = _lib.load()
+        w1, w2, saved = ctx.saved_tensors
+        need_x, need_w1, need_w2 = ctx.needs_input_grad[:3]
         dh = _matrix(dh)
         m, n = dh.shape
-        dtype = fp8._dtype_code(dh.dtype, "dh")
-        if ctx.keep == "inputs":
-            x, w1, w2 = ctx.saved_tensors
-        else:
-            w1, w2, qg, sg, qu, su, qx, sx = ctx.saved_tensors
         k = w1.shape[1]
-        need_x, need_w1, need_w2 = ctx.needs_input_grad[:3]
+        device = dh.device
         if m == 0:
             return (dh.new_empty((0, k)) if need_x else None, torch.zeros_like(w1) if need_w1 else None,
                     torch.zeros_like(w2) if need_w2 else None, None, None)
-        dg, du = torch.empty((m, n), dtype=dh.dtype, device=dh.device), torch.empty((m, n), dtype=dh.dtype, device=dh.device)
+        make = lambda need, rows: torch.empty((rows, k), dtype=dh.dtype, device=device) if need else None  # noqa: E731
+        dx, dw1, dw2 = make(need_x, m), make(need_w1, n), make(need_w2, n)
+        address = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        pitch = fp8._row_pitch
         if ctx.keep == "inputs":
-            _lib.check(lib.b200_gated_grad_hidden(*_mat(x), *_mat(w1), *_mat(w2), dtype, ctx.act, *_mat(dh), dg.data_ptr(),
-                                                  du.data_ptr(), n, m, n, k, *_stream(dh), None))
+            source = (saved.data_ptr(), pitch(saved), None, 0, 0)
+            nbytes = 4 * m * n
         else:
-            _lib.check(lib.b200_gated_grad_hidden_kept(qg.data_ptr(), qu.data_ptr(), fp8._row_pitch(qg), sg.data_ptr(),
-                                                       su.data_ptr(), sg.stride(0), sg.stride(1), dtype, ctx.act, *_mat(dh),
-                                                       dg.data_ptr(), du.data_ptr(), n, m, n, *_stream(dh)))
-        dx = dw1 = dw2 = None
-        if need_x:
-            dx = torch.empty((m, k), dtype=dh.dtype, device=dh.device)
-            _lib.check(lib.b200_gated_grad_input(dg.data_ptr(), du.data_ptr(), n, *_mat(w1), *_mat(w2), dtype, dx.data_ptr(), k,
-                                                 m, n, k, *_stream(dh), None))
-        if need_w1 or need_w2:
-            if ctx.keep == "fp8":
-                x = fp8.dequantize_fp8(qx, sx, dh.dtype)
-            dw1 = torch.empty((n, k), dtype=dh.dtype, device=dh.device)
-            dw2 = torch.empty((n, k), dtype=dh.dtype, device=dh.device)
-            _lib.check(lib.b200_gated_grad_weight(dg.data_ptr(), du.data_ptr(), n, *_mat(x), dtype, dw1.data_ptr(),
-                                                  dw2.data_ptr(), k, m, n, k, *_stream(dh), None))
-        return dx, dw1 if need_w1 else None, dw2 if need_w2 else None, None, None
+            source = (None, 0, saved.data_ptr(), saved.numel(), saved.numel() != _kept_bytes(m, n, k, False))
+            nbytes = 4 * m * n + 2 * m * k
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        code = _lib.load().b200_gated_backward(*source, w1.data_ptr(), pitch(w1), w2.data_ptr(), pitch(w2), fp8._DTYPES[dh.dtype],
+                                               ctx.act, dh.data_ptr(), pitch(dh), address(dx), k, address(dw1), address(dw2), k,
+                                               m, n, k, scratch.data_ptr(), nbytes, fp8._raw_stream(device.index),
+                                               device.index, None)
+        if code:
+            _lib.check(code)
+        return dx, dw1, dw2, None, None
 
 
 def gated_ffn(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, *, activation: str = "silu", keep: str = "inputs") -> torch.Tensor:
@@ -139,5 +149,5 @@ def gated_ffn(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, *, activation
     if torch.is_grad_enabled() and (x.requires_grad or w1.requires_grad or w2.requires_grad):
         h = _GatedFfn.apply(x2, w1, w2, act, keep)
     else:
-        h = _forward(x2, w1, w2, act, None)
+        h = _forward(x2, w1, w2, act, None, False)
     return h if x.dim() == 2 else h.view(*lead, w1.shape[0])

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 FAKE = 0x7F0000000000  # 16-byte aligned fake device address; never dereferenced on the host
-NULL, SHAPE, ALIGN, VARIANT, LIMIT = -1, -2, -3, -5, -7
+NULL, SHAPE, ALIGN, WORKSPACE, VARIANT, LIMIT = -1, -2, -3, -4, -5, -7
 
 
 @pytest.fixture(scope="module")
@@ -88,48 +88,63 @@ def _gated_args(kw):
 def test_gated_forward_refusals(lib, kw, code, needle):
     v = _gated_args(kw)
     _rejected(lib, lib.b200_gated_forward(v["x"], v["ldx"], v["w1"], v["ldw"], v["w2"], v["ldw"], v["dtype"], v["act"], v["out"], v["ld_out"],
-                                          None, None, 0, None, None, 0, 0, v["m"], v["n"], v["k"], None, 0, None), code, needle)
+                                          None, 0, 0, v["m"], v["n"], v["k"], None, 0, None), code, needle)
 
 
-def test_gated_forward_kept_copies_refusals(lib):
-    def f(qg=FAKE, qu=FAKE, ldq=128, sg=FAKE, su=FAKE):
-        return lib.b200_gated_forward(FAKE, 64, FAKE, 64, FAKE, 64, 1, 0, FAKE, 128, qg, qu, ldq, sg, su, 1, 4, 4, 128, 64, None, 0, None)
-    _rejected(lib, f(qu=None), NULL, "qu is NULL")
-    _rejected(lib, f(sg=None), NULL, "scales")
-    _rejected(lib, f(ldq=136), ALIGN, "qg")
-    _rejected(lib, f(qg=FAKE + 8), ALIGN, "qg must be")
+def test_gated_kept_buffer(lib, pkg):
+    size = lib.b200_gated_kept_bytes
+    for m, n, k in ((4, 128, 64), (7, 136, 200), (1, 8, 8)):
+        for keep_x in (0, 1):
+            assert size(m, n, k, keep_x) == pkg.gated._kept_bytes(m, n, k, bool(keep_x))
+        assert size(m, n, k, 1) > size(m, n, k, 0)
+    assert size(0, 128, 64, 1) == 0
+    f = lambda kept, nbytes, keep_x: lib.b200_gated_forward(FAKE, 64, FAKE, 64, FAKE, 64, 1, 0, FAKE, 128, kept, nbytes, keep_x,  # noqa: E731
+                                                            4, 128, 64, None, 0, None)
+    _rejected(lib, f(FAKE, size(4, 128, 64, 1) - 1, 1), WORKSPACE, str(size(4, 128, 64, 1)))
+    _rejected(lib, f(FAKE, size(4, 128, 64, 0) - 1, 0), WORKSPACE, str(size(4, 128, 64, 0)))
+    _rejected(lib, f(FAKE + 8, 1 << 20, 1), WORKSPACE, "aligned")
 
 
-@pytest.mark.parametrize("kw,code,needle", GATED_BAD)
-def test_gated_grad_hidden_refusals(lib, kw, code, needle):
-    v = _gated_args(kw)
-    _rejected(lib, lib.b200_gated_grad_hidden(v["x"], v["ldx"], v["w1"], v["ldw"], v["w2"], v["ldw"], v["dtype"], v["act"], FAKE, 128,
-                                              v["out"], v["out"], v["ld_out"], v["m"], v["n"], v["k"], None, 0, None), code, needle)
+def _backward(lib, **kw):
+    v = dict(x=FAKE, ldx=64, kept=None, kept_bytes=0, keep_x=0, w1=FAKE, w2=FAKE, ldw=64, dtype=1, act=0, dh=FAKE, ld_dh=128, dx=FAKE, ld_dx=64,
+             dw1=FAKE, dw2=FAKE, ld_dw=64, m=4, n=128, k=64, scratch=FAKE, nbytes=1 << 20)
+    v.update(kw)
+    return lib.b200_gated_backward(v["x"], v["ldx"], v["kept"], v["kept_bytes"], v["keep_x"], v["w1"], v["ldw"], v["w2"], v["ldw"], v["dtype"],
+                                   v["act"], v["dh"], v["ld_dh"], v["dx"], v["ld_dx"], v["dw1"], v["dw2"], v["ld_dw"], v["m"], v["n"],
+                                   v["k"], v["scratch"], v["nbytes"], None, 0, None)
 
 
-def test_gated_other_gradient_refusals(lib):
-    kept = lambda qg=FAKE, ldq=128, sg=FAKE, act=0, dh=FAKE, ld=128, n=128, m=4: lib.b200_gated_grad_hidden_kept(  # noqa: E731
-        qg, FAKE, ldq, sg, FAKE, 1, 4, 1, act, dh, ld, FAKE, FAKE, 128, m, n, None, 0)
-    _rejected(lib, kept(qg=None), NULL, "qg is NULL")
-    _rejected(lib, kept(sg=None), NULL, "scale")
-    _rejected(lib, kept(act=5), VARIANT, "activation 5")
-    _rejected(lib, kept(n=100), SHAPE, "n=100")
-    _rejected(lib, kept(m=0), SHAPE, "positive")
-    _rejected(lib, kept(ldq=120), ALIGN, "of qg")
-    _rejected(lib, kept(ld=100), ALIGN, "of dh")
-    dx = lambda dg=FAKE, ld=128, ldw=64, out=FAKE, ldo=64, m=4, n=128, k=64, dtype=1: lib.b200_gated_grad_input(  # noqa: E731
-        dg, FAKE, ld, FAKE, ldw, FAKE, ldw, dtype, out, ldo, m, n, k, None, 0, None)
-    dw = lambda dg=FAKE, ld=128, ldw=64, out=FAKE, ldo=64, m=4, n=128, k=64, dtype=1: lib.b200_gated_grad_weight(  # noqa: E731
-        dg, FAKE, ld, FAKE, ldw, dtype, out, FAKE, ldo, m, n, k, None, 0, None)
-    for f in (dx, dw):
-        _rejected(lib, f(dg=None), NULL, "dg is NULL")
-        _rejected(lib, f(out=None), NULL, "is NULL")
-        _rejected(lib, f(ld=100), ALIGN, "of dg")
-        _rejected(lib, f(ldw=60), ALIGN, "pitch 60")
-        _rejected(lib, f(ldo=60), ALIGN, "pitch 60")
-        _rejected(lib, f(m=0), SHAPE, "positive")
-        _rejected(lib, f(n=12), SHAPE, "n=12")
-        _rejected(lib, f(dtype=9), VARIANT, "dtype 9")
+@pytest.mark.parametrize("kw,code,needle", [
+    (dict(x=None), NULL, "x is NULL"), (dict(w1=None), NULL, "w1 is NULL"), (dict(w2=None), NULL, "w2 is NULL"), (dict(dh=None), NULL, "dh is NULL"),
+    (dict(dx=None, dw1=None, dw2=None), NULL, "no gradient"), (dict(dtype=4), VARIANT, "dtype 4"), (dict(act=2), VARIANT, "activation 2"),
+    (dict(m=0), SHAPE, "positive"), (dict(n=100), SHAPE, "n=100"), (dict(k=68), SHAPE, "k=68"), (dict(ldx=60), ALIGN, "of x"),
+    (dict(ldw=68), ALIGN, "of w1"), (dict(ld_dh=100), ALIGN, "of dh"), (dict(ld_dx=60), ALIGN, "of dx"), (dict(ld_dw=60), ALIGN, "of dw1"),
+    (dict(dw1=None, ld_dw=60), ALIGN, "of dw2"), (dict(dh=FAKE + 2), ALIGN, "dh must be"), (dict(scratch=None), WORKSPACE, "scratch"),
+    (dict(scratch=FAKE + 4), WORKSPACE, "aligned"), (dict(nbytes=4 * 4 * 128 - 1), WORKSPACE, "2048"),
+    (dict(kept=FAKE, kept_bytes=16, keep_x=1), WORKSPACE, "8-bit copies"), (dict(kept=FAKE, kept_bytes=1 << 20, keep_x=0), VARIANT, "keep_x"),
+    (dict(kept=FAKE, kept_bytes=1 << 20, keep_x=1, nbytes=4 * 4 * 128 + 2 * 4 * 64 - 1), WORKSPACE, "2560"),
+])
+def test_gated_backward_refusals(lib, kw, code, needle):
+    _rejected(lib, _backward(lib, **kw), code, needle)
+
+
+def test_fp8_linear_scratch(lib):
+    assert lib.b200_fp8_linear_scratch_bytes(16, 4096) == 0 and lib.b200_fp8_linear_scratch_bytes(0, 64) == 0
+    need = lib.b200_fp8_linear_scratch_bytes(17, 200)
+    assert need == 17 * 208 + 17 * 2 * 4
+    f = lambda m=17, x=FAKE, w=FAKE, sf=FAKE, y=FAKE, n=128, scratch=FAKE, nbytes=1 << 20, ldx=200, dtype=0: lib.b200_fp8_linear(  # noqa: E731
+        x, ldx, dtype, w, 208, sf, 2, 1, y, 128, m, n, 200, scratch, nbytes, None, 0, None)
+    _rejected(lib, f(nbytes=need - 1), WORKSPACE, str(need))
+    _rejected(lib, f(scratch=None), WORKSPACE, "scratch")
+    _rejected(lib, f(scratch=FAKE + 8), WORKSPACE, "aligned")
+    _rejected(lib, f(x=None), NULL, "NULL")
+    _rejected(lib, f(w=None), NULL, "w is NULL")
+    _rejected(lib, f(y=None), NULL, "y is NULL")
+    _rejected(lib, f(sf=None), NULL, "NULL")
+    _rejected(lib, f(n=4), SHAPE, "n=4")
+    _rejected(lib, f(m=0), SHAPE, "positive")
+    _rejected(lib, f(ldx=199), ALIGN, "ldx=199")
+    _rejected(lib, f(dtype=5), VARIANT, "dtype 5")
 
 
 def test_no_cpu_path(pkg):

@@ -125,7 +125,7 @@ def test_kept_copies_and_the_backward_pass_from_them(pkg, dense, m, n, k, dtype,
     x, w1, w2, dh = _inputs(m, n, k, dtype)
     leaves = [t.requires_grad_() for t in (x, w1, w2)]
     h = pkg.gated.gated_ffn(*leaves, activation=act, keep="fp8")
-    w1s, w2s, qg, sg, qu, su, qx, sx = h.grad_fn.saved_tensors
+    qg, sg, qu, su, qx, sx = pkg.gated.kept_copies(h.grad_fn.saved_tensors[2], m, n, k)
     grads = torch.autograd.grad(h, leaves, dh)
     with torch.no_grad():
         _within(h, *_forward_bound(dense, x, w1, w2, act), "h")
@@ -152,25 +152,25 @@ def test_kept_copies_and_the_backward_pass_from_them(pkg, dense, m, n, k, dtype,
 
 
 @pytest.mark.parametrize("m,n,k", [(5, 16, 24), (130, 72, 264), (300, 520, 200)])
-def test_gradient_products_are_exact_on_small_integers(pkg, m, n, k):
-    """Integers whose products and sums stay below 2^8: bf16 holds every result, so any difference is a mistake."""
-    g = torch.Generator(device="cuda").manual_seed(m)
+def test_gradients_are_exact_on_integers(pkg, m, n, k):
+    """g is an integer of at least 24 (a column of ones in x, 32 in w1): sigma(g) is 1 in fp32, act(g) = g and act' = 1, so dg = dh u
+    and du = dh g are integers below 2^8 and every sum behind dx and dw is exact in fp32: any difference is a mistake."""
+    r = torch.Generator(device="cuda").manual_seed(m)
+
     def ints(*s):
-        keep = torch.rand(s, generator=g, device="cuda") < 0.05
-        return (torch.randint(-2, 3, s, generator=g, device="cuda") * keep).to(BF16)
-    dg, du, x, w1, w2 = ints(m, n), ints(m, n), ints(m, k), ints(n, k), ints(n, k)
-    lib, st = pkg._lib.load(), torch.cuda.current_stream().cuda_stream
-    dx = torch.empty((m, k), dtype=BF16, device="cuda")
-    dw = torch.empty((2, n, k), dtype=BF16, device="cuda")
-    pkg._lib.check(lib.b200_gated_grad_input(dg.data_ptr(), du.data_ptr(), n, w1.data_ptr(), k, w2.data_ptr(), k, pkg._lib.DTYPE_BF16,
-                                             dx.data_ptr(), k, m, n, k, st, 0, None))
-    pkg._lib.check(lib.b200_gated_grad_weight(dg.data_ptr(), du.data_ptr(), n, x.data_ptr(), k, pkg._lib.DTYPE_BF16, dw[0].data_ptr(),
-                                              dw[1].data_ptr(), k, m, n, k, st, 0, None))
-    want = dg.double() @ w1.double() + du.double() @ w2.double()
-    assert want.abs().max() < 256 and torch.equal(dx.double(), want)
-    for got, d in zip(dw, (dg, du)):
-        want = d.double().t() @ x.double()
-        assert want.abs().max() < 256 and torch.equal(got.double(), want)
+        some = torch.rand(s, generator=r, device="cuda") < 0.02
+        return (torch.randint(-1, 2, s, generator=r, device="cuda") * some).to(BF16)
+
+    x, w1, w2 = ints(m, k), ints(n, k), ints(n, k)
+    x[:, 0], w1[:, 0], w2[:, 0] = 1, 32, 2
+    dh = torch.randint(-3, 4, (m, n), generator=r, device="cuda").to(BF16)
+    g, u = x.double() @ w1.double().t(), x.double() @ w2.double().t()
+    assert g.min() >= 24 and g.max() < 64 and u.abs().max() < 64
+    dg, du = dh.double() * u, dh.double() * g
+    want = (dg @ w1.double() + du @ w2.double(), dg.t() @ x.double(), du.t() @ x.double())
+    leaves = [t.requires_grad_() for t in (x, w1, w2)]
+    for got, y in zip(torch.autograd.grad(pkg.gated.gated_ffn(*leaves), leaves, dh), want):
+        assert y.abs().max() < 2 ** 24 and torch.equal(got, y.float().to(BF16))
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu"])
@@ -204,6 +204,11 @@ def test_only_what_is_asked_for(pkg, keep):
     for mask in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1), (0, 1, 1)):
         leaves = [t.clone().requires_grad_(bool(f)) for t, f in zip((x, w1, w2), mask)]
         got = torch.autograd.grad(pkg.gated.gated_ffn(*leaves, keep=keep), [t for t in leaves if t.requires_grad], dh)
+        for a, b in zip(got, [w for w, f in zip(want, mask) if f]):
+            assert torch.equal(a, b)
+        # the same gradients out of a block that could have given all
+        h = pkg.gated.gated_ffn(*full, keep=keep)
+        got = torch.autograd.grad(h, [t for t, f in zip(full, mask) if f], dh)
         for a, b in zip(got, [w for w, f in zip(want, mask) if f]):
             assert torch.equal(a, b)
 
