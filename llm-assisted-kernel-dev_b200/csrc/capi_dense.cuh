@@ -30,9 +30,9 @@ template <FfMode kMode> int opt_in_ff() {
     return rc ? rc : opt_in_smem(ff_gemm_pair<kMode, true>, kFfSmemBytes);
 }
 
-template <FewOp kOp, int kTokens> int opt_in_few() {
-    int rc = opt_in_smem(few_tokens_gemm<kOp, kTokens, false>, few_smem_bytes<kOp, kTokens>());
-    return rc ? rc : opt_in_smem(few_tokens_gemm<kOp, kTokens, true>, few_smem_bytes<kOp, kTokens>());
+template <FewOp kOp, int kTokens, bool kFuse = false> int opt_in_few() {
+    int rc = opt_in_smem(few_tokens_gemm<kOp, kTokens, false, kFuse>, few_smem_bytes<kOp, kTokens, kFuse>());
+    return rc ? rc : opt_in_smem(few_tokens_gemm<kOp, kTokens, true, kFuse>, few_smem_bytes<kOp, kTokens, kFuse>());
 }
 template <FewOp kOp> int opt_in_few_all() {
     int rc;
@@ -61,8 +61,7 @@ struct DenseCall {
         if ((rc = opt_in_smem(fp8_gemm_pair<true>, kFp8SmemBytes))) return;
         if ((rc = opt_in_few_all<FewOp::Few8>())) return;
         if ((rc = opt_in_few_all<FewOp::FewGated>())) return;
-        if ((rc = opt_in_smem(few_tokens_gemm<FewOp::Few8, 16, false, true>, few_smem_bytes<FewOp::Few8, 16>()))) return;
-        if ((rc = opt_in_smem(few_tokens_gemm<FewOp::Few8, 16, true, true>, few_smem_bytes<FewOp::Few8, 16>()))) return;
+        if ((rc = opt_in_few<FewOp::Few8, 16, true>())) return;
         if ((rc = opt_in_ff<FfMode::Forward>())) return;
         if ((rc = opt_in_ff<FfMode::GradHidden>())) return;
         if ((rc = opt_in_ff<FfMode::GradInput>())) return;
@@ -143,14 +142,14 @@ int few_splits(long long tiles, int steps, int slots) {
 }
 
 template <FewOp kOp, int kTokens, bool kBf16, bool kFuse = false> int launch_few_as(FewProblem& p, DenseCall& call) {
-    using S = FewShape<kOp, kTokens>;
+    using S = FewShape<kOp, kTokens, kFuse>;
     const int tiles = (p.n + 127) / 128, token_tiles = (p.m + kTokens - 1) / kTokens;
     const int splits = few_splits(static_cast<long long>(tiles) * token_tiles, p.steps, call.st->sm_count * S::kCtasPerSm);
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
     cfg.gridDim = dim3(tiles * splits, token_tiles, 1);
-    cfg.blockDim = dim3(kFuse ? kFewFuseThreads : kFewThreads, 1, 1);
-    cfg.dynamicSmemBytes = few_smem_bytes<kOp, kTokens>();
+    cfg.blockDim = dim3(S::kThreads, 1, 1);
+    cfg.dynamicSmemBytes = few_smem_bytes<kOp, kTokens, kFuse>();
     cfg.stream = call.stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -12,7 +12,8 @@
 //             memory (up to 16 tokens: every tile of W repeats that work, and a launch of its own costs more)
 //   FewGated  16-bit: g and u of the same rows and tokens side by side in tensor memory, h formed after the exchange
 //
-// Seven warps: 0-3 sums and results, 4 MMA issuer, 5 weight loads, 6 token loads (and their scales); 7-10 quantise (kFuse).
+// Warps: four or eight for sums and results, then MMA issuer, weight loads, token loads (and their scales), and four that
+// quantise (kFuse).
 #pragma once
 
 #include "dense_tiles.cuh"
@@ -39,11 +40,14 @@ struct FewProblem {
     uint32_t* status;
 };
 
-template <FewOp kOp, int kTokens> struct FewShape {
+template <FewOp kOp, int kTokens, bool kFuse> struct FewShape {
     static constexpr bool kFp8 = kOp == FewOp::Few8;
     static constexpr uint32_t kWeightBytes = (kFp8 ? 1u : 2u) * 16384u;     // 128 rows x 128 bytes of each weight
     static constexpr uint32_t kTokenBytes = kTokens * 128u;
     static constexpr uint32_t kStageBytes = kWeightBytes + kTokenBytes;
+    // warps that add up the blocks' sums: two for each quadrant of tensor memory with 128 tokens, half of them each
+    static constexpr int kSumWarps = kFp8 && kTokens == 128 ? 8 : 4;
+    static constexpr int kThreads = 32 * (kSumWarps + (kFuse ? 7 : 3));
     // two CTAs on an SM up to 64 (fp8) or 32 tokens, one beyond: registers and stages
     static constexpr int kCtasPerSm = kTokens <= (kFp8 ? 64 : 32) ? 2 : 1;
     static constexpr int kStages = static_cast<int>((kCtasPerSm == 2 ? 108u * 1024u : 200u * 1024u) / kStageBytes);
@@ -52,20 +56,18 @@ template <FewOp kOp, int kTokens> struct FewShape {
     static_assert((kFp8 ? 1u : 2u) * kTokens * 512u <= kStages * kStageBytes, "exchange area");
     static_assert(kStageBytes % 1024 == 0, "stages keep the alignment of the swizzle");
 };
-template <FewOp kOp, int kTokens> struct FewControl {
-    using S = FewShape<kOp, kTokens>;
+template <FewOp kOp, int kTokens, bool kFuse> struct FewControl {
+    using S = FewShape<kOp, kTokens, kFuse>;
     uint64_t wfull[S::kStages], tfull[S::kStages], empty[S::kStages];
     uint64_t sfull[S::kStages], sempty[S::kStages];
     uint64_t acc_full[2], acc_release[2];
     uint32_t tmem_base, abort_flag;
     alignas(16) float scale[S::kStages][kTokens];
 };
-template <FewOp kOp, int kTokens> constexpr uint32_t few_smem_bytes() {
-    using S = FewShape<kOp, kTokens>;
-    return 1024u + S::kStages * S::kStageBytes + sizeof(FewControl<kOp, kTokens>);
+template <FewOp kOp, int kTokens, bool kFuse> constexpr uint32_t few_smem_bytes() {
+    using S = FewShape<kOp, kTokens, kFuse>;
+    return 1024u + S::kStages * S::kStageBytes + sizeof(FewControl<kOp, kTokens, kFuse>);
 }
-constexpr int kFewThreads = 224, kFewFuseThreads = 352;
-constexpr int kFuseAhead = 4;            // blocks of k whose tokens a quantising half-warp loads at a time
 
 __device__ __forceinline__ float4 ld_cluster_v4f(uint32_t cluster_addr) {
     float4 v;
@@ -90,15 +92,18 @@ template <int kN> __device__ __forceinline__ void tc_ld_cols(uint32_t taddr, uin
 }
 
 template <FewOp kOp, int kTokens, bool kBf16, bool kFuse = false>
-__global__ void __launch_bounds__(kFuse ? kFewFuseThreads : kFewThreads, FewShape<kOp, kTokens>::kCtasPerSm)
+__global__ void __launch_bounds__(FewShape<kOp, kTokens, kFuse>::kThreads, FewShape<kOp, kTokens, kFuse>::kCtasPerSm)
 few_tokens_gemm(const __grid_constant__ FewProblem p) {
-    using S = FewShape<kOp, kTokens>;
+    using S = FewShape<kOp, kTokens, kFuse>;
     constexpr bool kFp8 = S::kFp8;
     constexpr int kStages = S::kStages;
-    constexpr int kChunk = kTokens < 32 ? kTokens : 32;
+    constexpr int kSumWarps = S::kSumWarps, kMma = kSumWarps, kLoadW = kSumWarps + 1, kLoadX = kSumWarps + 2;
+    constexpr int kMine = kTokens * 4 / kSumWarps;        // tokens of one summing warp
+    constexpr int kChunk = kMine < 32 ? kMine : 32;
+    constexpr int kFuseAhead = 4;                         // blocks of k whose tokens a quantising half-warp loads at a time
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    auto* ctl = reinterpret_cast<FewControl<kOp, kTokens>*>(smem_raw + (smem_base - smem_u32(smem_raw)) + kStages * S::kStageBytes);
+    auto* ctl = reinterpret_cast<FewControl<kOp, kTokens, kFuse>*>(smem_raw + (smem_base - smem_u32(smem_raw)) + kStages * S::kStageBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t splits;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
@@ -114,17 +119,17 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
             mbar_init(smem_u32(&ctl->tfull[s]), kFuse ? 4 : 1);       // kFuse: the quantising warps
             mbar_init(smem_u32(&ctl->empty[s]), 1);
             mbar_init(smem_u32(&ctl->sfull[s]), 32);
-            mbar_init(smem_u32(&ctl->sempty[s]), 4);
+            mbar_init(smem_u32(&ctl->sempty[s]), kSumWarps);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(smem_u32(&ctl->acc_full[b]), 1);
-            mbar_init(smem_u32(&ctl->acc_release[b]), 4);
+            mbar_init(smem_u32(&ctl->acc_release[b]), kSumWarps);
         }
         ctl->abort_flag = 0;
         fence_mbar_init();
         fence_proxy_async_smem();
     }
-    if (warp == 4) {
+    if (warp == kMma) {
         tmem_alloc(smem_u32(&ctl->tmem_base), S::kTmemCols);
         tmem_relinquish();
     }
@@ -133,14 +138,14 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
     tc_fence_after_sync();
     const uint32_t tmem_base = ctl->tmem_base;
     griddep_launch_dependents();   // after this CTA has its tensor memory: a CTA of the next kernel cannot take it away
-    if (!(warp == 5 && p.weights_early)) griddep_wait();
+    if (!(warp == kLoadW && p.weights_early)) griddep_wait();
 
-    float sum[kFp8 ? kTokens : 1];      // Few8: this lane's weight row, all tokens
+    float sum[kFp8 ? kMine : 1];        // Few8: this lane's weight row, this warp's tokens
     bool ok = true;
-    if (kFuse && (warp == 6 || warp >= 7)) {
+    if (kFuse && warp >= kLoadX) {
         // ------------------------------ tokens: quantised here (a half-warp holds one token's block of 128)
-        if (warp >= 7) {
-            const int half = (warp - 7) * 2 + (lane >> 4), l = lane & 15;
+        if (warp > kLoadX) {
+            const int half = (warp - kLoadX - 1) * 2 + (lane >> 4), l = lane & 15;
             uint32_t s = 0, ph = 0;
             for (int i0 = 0; ok && i0 < count; i0 += kFuseAhead) {
                 uint4 v[kFuseAhead][kTokens / 8];
@@ -187,18 +192,18 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
             }
         }
         __syncwarp();
-    } else if (warp == 5 || warp == 6) {
+    } else if (warp == kLoadW || warp == kLoadX) {
         // ------------------------------ loads
         uint32_t s = 0, ph = 0;
         for (int i = 0; i < count; ++i) {
             ok = mbar_wait<true>(smem_u32(&ctl->empty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense);
-            if (kFp8 && warp == 6 && ok)
+            if (kFp8 && warp == kLoadX && ok)
                 ok = mbar_wait<true>(smem_u32(&ctl->sempty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const uint32_t dst = smem_base + s * S::kStageBytes;
             const int k0 = (begin + i) * (kFp8 ? 128 : 64);
-            if (warp == 5) {
+            if (warp == kLoadW) {
                 const uint32_t bar = smem_u32(&ctl->wfull[s]);
                 mbar_arrive_expect_tx_elect(bar, S::kWeightBytes);
                 tma_load_2d_elect(dst, &p.w[0], bar, k0, w_row);
@@ -219,11 +224,11 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
             }
             if (++s == kStages) { s = 0; ph ^= 1u; }
         }
-        if (kFp8 && warp == 6) asm volatile("cp.async.wait_all;" ::: "memory");
+        if (kFp8 && warp == kLoadX) asm volatile("cp.async.wait_all;" ::: "memory");
         if (!ok)
             for (int i = 0; i < 64; ++i) __nanosleep(2000);   // error path: let copies in flight land
         __syncwarp();
-    } else if (warp == 4) {
+    } else if (warp == kMma) {
         // ------------------------------ MMA issuer
         constexpr uint32_t kIdesc = idesc_dense(128, kTokens, kFp8 ? 0u : (kBf16 ? 1u : 0u), false, false);
         uint32_t s = 0, ph = 0;
@@ -255,13 +260,13 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
         __syncwarp();
     } else if constexpr (kFp8) {
         // ------------------------------ sums of the blocks
-        uint64_t acc[kTokens / 2];
+        uint64_t acc[kMine / 2];
 #pragma unroll
-        for (int j = 0; j < kTokens / 2; ++j) acc[j] = 0;
+        for (int j = 0; j < kMine / 2; ++j) acc[j] = 0;
         const bool exists = w_row < p.n;
         const float* sb = p.sfb + (w_row / kFp8Block) * p.sfb_row + begin * p.sfb_col;
         float b_next = exists && count > 0 ? sb[0] : 0.0f;
-        const uint32_t lanes = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
+        const uint32_t lanes = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + (warp >> 2) * kMine;
         uint32_t s = 0, ph = 0;
         for (int i = 0; i < count; ++i) {
             const uint64_t b2 = pack_f32x2(__float_as_uint(b_next), __float_as_uint(b_next));
@@ -271,9 +276,9 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
                  mbar_wait_converged(smem_u32(&ctl->acc_full[i & 1]), (i >> 1) & 1, abort_flag, p.status, kStatusDense);
             if (!ok) break;
             tc_fence_after_sync();
-            const uint32_t scales = smem_u32(&ctl->scale[s][0]);
+            const uint32_t scales = smem_u32(&ctl->scale[s][(warp >> 2) * kMine]);
 #pragma unroll
-            for (int c = 0; c < kTokens / kChunk; ++c) {
+            for (int c = 0; c < kMine / kChunk; ++c) {
                 uint32_t v[kChunk];
                 tc_ld_cols<kChunk>(lanes + (i & 1) * kTokens + c * kChunk, v);
                 tc_wait_ld();
@@ -293,7 +298,7 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
             if (++s == kStages) { s = 0; ph ^= 1u; }
         }
 #pragma unroll
-        for (int j = 0; j < kTokens / 2; ++j) {
+        for (int j = 0; j < kMine / 2; ++j) {
             const float2 two = unpack_f32x2(acc[j]);
             sum[2 * j] = two.x;
             sum[2 * j + 1] = two.y;
@@ -305,15 +310,16 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
 
     // ------------------------------ results
     const int tokens = p.m - token0 < kTokens ? p.m - token0 : kTokens;
-    const int row = w_row + warp * 32 + lane;                       // consumers: this lane's weight row = column of C
-    const uint32_t area = smem_base + (warp * 32 + lane) * 4;       // exchange: [g | u][token][128 rows]
+    const int row = w_row + (warp & 3) * 32 + lane;                 // summing warps: this lane's weight row = column of C
+    const int first = (warp >> 2) * kMine;                          // and first token
+    const uint32_t area = smem_base + ((warp & 3) * 32 + lane) * 4; // exchange: [g | u][token][128 rows]
     uint16_t* out = p.c + token0 * p.ldc + row;
     if (splits == 1) {
-        if (warp < 4 && ok) {
+        if (warp < kSumWarps && ok) {
             if constexpr (kFp8) {
 #pragma unroll
-                for (int t = 0; t < kTokens; ++t)
-                    if (t < tokens && row < p.n) out[t * p.ldc] = to_16<kBf16>(sum[t]);
+                for (int t = 0; t < kMine; ++t)
+                    if (first + t < tokens && row < p.n) out[(first + t) * p.ldc] = to_16<kBf16>(sum[t]);
             } else {
                 const uint32_t acc = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
 #pragma unroll 1
@@ -332,11 +338,11 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
         }
     } else {
         // every stage has been consumed (the last accumulator is complete): its memory now holds the partial sums
-        if (warp < 4 && ok) {
+        if (warp < kSumWarps && ok) {
             if constexpr (kFp8) {
 #pragma unroll
-                for (int t = 0; t < kTokens; ++t)
-                    if (t < tokens) st_shared_f32(area + t * 512, sum[t]);
+                for (int t = 0; t < kMine; ++t)
+                    if (first + t < tokens) st_shared_f32(area + (first + t) * 512, sum[t]);
             } else {
                 const uint32_t acc = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
 #pragma unroll 1
@@ -360,9 +366,9 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
         // token t is summed by rank t % splits, in rank order; a lane takes four neighbouring columns of C, and all
         // ranks' loads are in flight before the first is added (one remote load takes about 0.3 us)
         const int col = w_row + lane * 4;
-        if (warp < 4 && col < p.n) {
+        if (warp < kSumWarps && col < p.n) {
 #pragma unroll 2
-            for (int t = rank + splits * warp; t < tokens; t += splits * 4) {
+            for (int t = rank + splits * warp; t < tokens; t += splits * kSumWarps) {
                 const uint32_t mine = smem_base + t * 512 + lane * 16;
                 float4 g[8], u[kFp8 ? 1 : 8];
 #pragma unroll
@@ -393,7 +399,7 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
     }
     tc_fence_before_sync();
     __syncthreads();
-    if (warp == 4) {
+    if (warp == kMma) {
         tc_fence_after_sync();
         tmem_dealloc(tmem_base, S::kTmemCols);
     }

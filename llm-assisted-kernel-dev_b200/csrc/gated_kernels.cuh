@@ -18,7 +18,7 @@
 //
 // Bound by the tensor cores.  A 256 x 256 x 64 step of a pair takes 512 clocks of MMA at 4096 multiply-adds
 // per clock and SM; per SM it reads 32 KB by TMA (64 B/clk; this GPU feeds ~98) and 32 KB by MMA.
-// Six warps: 0-3 epilogue (each its 32 accumulator rows), 4 MMA issuer (first CTA), 5 TMA producer.
+// Ten warps: 0-7 epilogue (quadrant w % 4, one half of the columns each), 8 MMA issuer (first CTA), 9 TMA producer.
 #pragma once
 
 #include "dense_tiles.cuh"
@@ -42,11 +42,11 @@ struct FfProblem {
     uint32_t* status;
 };
 
-constexpr int kFfStages = 6;
+constexpr int kFfStages = 5;
 constexpr uint32_t kFfOperandBytes = 128u * 128u;            // 128 rows x 64 k (K-major) or 2 boxes of 64 x 64 (MN-major)
 constexpr uint32_t kFfStageBytes = 2u * kFfOperandBytes;
-constexpr uint32_t kFfStagingBytes = 4u * 8192u;             // per epilogue warp two boxes of 32 rows x 128 bytes
-constexpr int kFfThreads = 192;
+constexpr uint32_t kFfStagingBytes = 8u * 8192u;             // per epilogue warp two boxes of 32 rows x 128 bytes
+constexpr int kFfThreads = 320;
 
 struct FfControl {
     uint64_t full[kFfStages], empty[kFfStages];
@@ -75,25 +75,22 @@ template <bool kSlope> __device__ __forceinline__ GateValue gate(float z, int ge
     return r;
 }
 
-// h = act(g) u of 32 rows x 128 columns.
+// h = act(g) u of 32 rows x 64 columns (`acc` and `col`: this warp's half).
 template <bool kBf16>
 __device__ __forceinline__ void ff_epilogue_forward(const FfProblem& p, uint32_t acc, BoxWriter& w, int row, int col) {
+    const uint32_t box = w.acquire();
 #pragma unroll 1
-    for (int half = 0; half < 2; ++half) {
-        const uint32_t box = w.acquire();
-#pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-            uint32_t g[32], u[32];
-            tc_ld_x32(acc + half * 64 + c * 32, g);
-            tc_ld_x32(acc + 128 + half * 64 + c * 32, u);
-            tc_wait_ld();
-            float f[32];
+    for (int c = 0; c < 2; ++c) {
+        uint32_t g[32], u[32];
+        tc_ld_x32(acc + c * 32, g);
+        tc_ld_x32(acc + 128 + c * 32, u);
+        tc_wait_ld();
+        float f[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] = gate<false>(__uint_as_float(g[i]), p.gelu).value * __uint_as_float(u[i]);
-            put_chunk<kBf16>(w, box, c * 4, f);
-        }
-        w.send(box, &p.out[0], col + half * 64, row, row < p.rows && col + half * 64 < p.cols);
+        for (int i = 0; i < 32; ++i) f[i] = gate<false>(__uint_as_float(g[i]), p.gelu).value * __uint_as_float(u[i]);
+        put_chunk<kBf16>(w, box, c * 4, f);
     }
+    w.send(box, &p.out[0], col, row, row < p.rows && col < p.cols);
 }
 
 // 8-bit copy of one projection's 32 rows x 128 columns (a lane holds a whole block: its row's 128 columns).
@@ -127,56 +124,53 @@ __device__ __forceinline__ void ff_epilogue_keep(const FfProblem& p, int which, 
     if (r < p.rows && col < p.cols) p.sf[which][r * p.sf_row + (col / kFp8Block) * p.sf_col] = s.scale;
 }
 
-// dg and du of 32 rows x 128 columns from the accumulators and dh.
+// dg and du of 32 rows x 64 columns from the accumulators and dh (`acc` and `col`: this warp's half).
 template <bool kBf16>
-__device__ __forceinline__ void ff_epilogue_grad_hidden(const FfProblem& p, uint32_t acc, BoxWriter& w, int row, int col) {
-    const int r = row + w.lane;
+__device__ __forceinline__ void ff_load_dh(const FfProblem& p, int row, int col, int lane, uint4 (&d)[8]) {
+    const int r = row + lane;
     const uint16_t* dh = p.dh + r * p.ld_dh + col;
-#pragma unroll 1
-    for (int half = 0; half < 2; ++half) {
-        const int c0 = half * 64;
-        // sixteen-byte pieces of this lane's dh row, 64 columns
-        uint4 d[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            d[j] = (r < p.rows && col + c0 + 8 * j < p.cols) ? *reinterpret_cast<const uint4*>(dh + c0 + 8 * j)
-                                                             : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < 8; ++j)
+        d[j] = (r < p.rows && col + 8 * j < p.cols) ? *reinterpret_cast<const uint4*>(dh + 8 * j) : make_uint4(0, 0, 0, 0);
+}
+template <bool kBf16>
+__device__ __forceinline__ void ff_epilogue_grad_hidden(const FfProblem& p, uint32_t acc, BoxWriter& w, int row, int col,
+                                                        const uint4 (&d)[8]) {
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            const uint32_t box = w.acquire();
+    for (int which = 0; which < 2; ++which) {
+        const uint32_t box = w.acquire();
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t g[32], u[32];
-                tc_ld_x32(acc + c0 + c * 32, g);
-                if (which == 0) tc_ld_x32(acc + 128 + c0 + c * 32, u);
-                tc_wait_ld();
-                float f[32];
+        for (int c = 0; c < 4; ++c) {
+            uint32_t g[16], u[16];
+            tc_ld_x16(acc + c * 16, g);
+            if (which == 0) tc_ld_x16(acc + 128 + c * 16, u);
+            tc_wait_ld();
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float e[8];
-                    to_float8<kBf16>(d[c * 4 + j], e);
+            for (int j = 0; j < 2; ++j) {
+                float e[8], f[8];
+                to_float8<kBf16>(d[c * 2 + j], e);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int at = 8 * j + i;
-                        if (which == 0)
-                            f[at] = e[i] * __uint_as_float(u[at]) * gate<true>(__uint_as_float(g[at]), p.gelu).slope;
-                        else
-                            f[at] = e[i] * gate<false>(__uint_as_float(g[at]), p.gelu).value;
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    const int at = 8 * j + i;
+                    if (which == 0)
+                        f[i] = e[i] * __uint_as_float(u[at]) * gate<true>(__uint_as_float(g[at]), p.gelu).slope;
+                    else
+                        f[i] = e[i] * gate<false>(__uint_as_float(g[at]), p.gelu).value;
                 }
-                put_chunk<kBf16>(w, box, c * 4, f);
+                w.put(box, c * 2 + j, pack_16<kBf16>(f[0], f[1]), pack_16<kBf16>(f[2], f[3]), pack_16<kBf16>(f[4], f[5]),
+                      pack_16<kBf16>(f[6], f[7]));
             }
-            w.send(box, &p.out[which], col + c0, row, row < p.rows && col + c0 < p.cols);
         }
+        w.send(box, &p.out[which], col, row, row < p.rows && col < p.cols);
     }
 }
 
-// 32 rows x 256 columns of a plain product.
+// 32 rows x 128 columns of a plain product.
 template <bool kBf16>
 __device__ __forceinline__ void ff_epilogue_plain(const FfProblem& p, const CUtensorMap* map, uint32_t acc, BoxWriter& w,
                                                   int row, int col) {
 #pragma unroll 1
-    for (int part = 0; part < 4; ++part) {
+    for (int part = 0; part < 2; ++part) {
         const uint32_t box = w.acquire();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -215,14 +209,14 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(smem_u32(&ctl->acc_full[b]), 1);
-            mbar_init(smem_u32(&ctl->acc_release[b]), 8);    // four epilogue warps of each CTA; used in the first
+            mbar_init(smem_u32(&ctl->acc_release[b]), 16);   // eight epilogue warps of each CTA; used in the first
         }
         mbar_init(smem_u32(&ctl->done), 1);
         ctl->abort_flag = 0;
         fence_mbar_init();
         fence_proxy_async_smem();
     }
-    if (warp == 4) {
+    if (warp == 8) {
         tmem_alloc_pair(smem_u32(&ctl->tmem_base), 512);
         tmem_relinquish_pair();
     }
@@ -235,7 +229,7 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
     griddep_launch_dependents();   // after this CTA has its tensor memory: a CTA of the next kernel cannot take it away
     griddep_wait();
 
-    if (warp == 5) {
+    if (warp == 9) {
         // ------------------------------ producer: this CTA's rows of A and its half of B
         uint32_t s = 0, ph = 0;
         bool ok = true;
@@ -272,7 +266,7 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
         if (!ok)
             for (int i = 0; i < 64; ++i) __nanosleep(2000);   // error path: let copies in flight land
         __syncwarp();
-    } else if (warp == 4) {
+    } else if (warp == 8) {
         // ------------------------------ MMA issuer
         if (rank == 0) {
             constexpr uint32_t kIdesc = idesc_dense(256, 256, kBf16 ? 1u : 0u, kAMn, kBMn);
@@ -309,28 +303,29 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
         __syncwarp();
     } else {
         // ------------------------------ epilogue
+        const int quad = warp & 3, half = warp >> 2;
         BoxWriter w{smem_base + kFfStages * kFfStageBytes + static_cast<uint32_t>(warp) * 8192u, lane, 0};
+        const uint32_t release = map_to_cta(smem_u32(&ctl->acc_release[0]), 0);
         int it = 0;
         for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, p.batches); t.valid(); t.next(), ++it) {
-            if (!__all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->acc_full[it & 1]), (it >> 1) & 1, abort_flag, p.status, kStatusDense)))
-                break;
+            const int row = t.m * 256 + static_cast<int>(rank) * 128 + quad * 32;
+            const int col = t.n * kTileCols + half * (kTileCols / 2);
+            uint4 d[8];
+            if constexpr (kMode == FfMode::GradHidden) ff_load_dh<kBf16>(p, row, col, lane, d);   // arrives while the products are formed
+            if (!mbar_wait_converged(smem_u32(&ctl->acc_full[it & 1]), (it >> 1) & 1, abort_flag, p.status, kStatusDense)) break;
             tc_fence_after_sync();
-            const uint32_t acc = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + (it & 1) * 256;
-            const int row = t.m * 256 + static_cast<int>(rank) * 128 + warp * 32, col = t.n * kTileCols;
+            const uint32_t acc = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + (it & 1) * 256;
             if constexpr (kMode == FfMode::Forward) {
-                ff_epilogue_forward<kBf16>(p, acc, w, row, col);
-                if (p.keep) {
-                    ff_epilogue_keep(p, 0, acc, w, row, col);
-                    ff_epilogue_keep(p, 1, acc + 128, w, row, col);
-                }
+                ff_epilogue_forward<kBf16>(p, acc + half * 64, w, row, col);
+                if (p.keep) ff_epilogue_keep(p, half, acc + half * 128, w, row, t.n * kTileCols);   // g by one half of the warps, u by the other
             } else if constexpr (kMode == FfMode::GradHidden) {
-                ff_epilogue_grad_hidden<kBf16>(p, acc, w, row, col);
+                ff_epilogue_grad_hidden<kBf16>(p, acc + half * 64, w, row, col, d);
             } else {
-                ff_epilogue_plain<kBf16>(p, &p.out[t.batch], acc, w, row, col);
+                ff_epilogue_plain<kBf16>(p, &p.out[t.batch], acc + half * 128, w, row, col);
             }
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&ctl->acc_release[it & 1]), 0));
+            mbar_arrive_cluster_relaxed_elect(release + 8 * (it & 1));
         }
         if (lane == 0) bulk_wait_group_read_all();
         __syncwarp();
@@ -340,7 +335,7 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
     __syncthreads();
     cluster_arrive();
     cluster_wait();
-    if (warp == 4) {
+    if (warp == 8) {
         tc_fence_after_sync();
         tmem_dealloc_pair(tmem_base, 512);
     }
