@@ -26,8 +26,11 @@ int encode_matrix_map(CUtensorMap* map, const void* base, int elem, long long co
 std::map<int, bool> g_dense_ready;   // devices whose kernels were given their shared memory
 
 template <FfMode kMode> int opt_in_ff() {
-    int rc = opt_in_smem(ff_gemm_pair<kMode, false>, kFfSmemBytes);
-    return rc ? rc : opt_in_smem(ff_gemm_pair<kMode, true>, kFfSmemBytes);
+    int rc;
+    if ((rc = opt_in_smem(ff_gemm_pair<kMode, false, 256>, ff_smem_bytes<256>()))) return rc;
+    if ((rc = opt_in_smem(ff_gemm_pair<kMode, true, 256>, ff_smem_bytes<256>()))) return rc;
+    if ((rc = opt_in_smem(ff_gemm_pair<kMode, false, 128>, ff_smem_bytes<128>()))) return rc;
+    return opt_in_smem(ff_gemm_pair<kMode, true, 128>, ff_smem_bytes<128>());
 }
 
 template <FewOp kOp, int kTokens, bool kFuse = false> int opt_in_few() {
@@ -126,12 +129,24 @@ int check_gated(const char* what, int dtype, int act, int m, int n, int k) {
     return 0;
 }
 
-template <FfMode kMode> int launch_ff(const char* name, FfProblem& p, int dtype, DenseCall& call, void* status) {
+template <FfMode kMode> int launch_ff(const char* name, FfProblem& p, int tile_n, int dtype, DenseCall& call, void* status) {
     p.status = status ? static_cast<uint32_t*>(status) : call.st->status;
     const int grid = pair_grid(static_cast<long long>(p.m_tiles) * p.n_tiles * p.batches, call.st->sm_count);
-    if (dtype == B200_DTYPE_BF16)
-        return launch_dense(name, ff_gemm_pair<kMode, true>, dim3(grid), kFfThreads, kFfSmemBytes, call.stream, p);
-    return launch_dense(name, ff_gemm_pair<kMode, false>, dim3(grid), kFfThreads, kFfSmemBytes, call.stream, p);
+    const bool bf16 = dtype == B200_DTYPE_BF16;
+    if (tile_n == 128)
+        return launch_dense(name, bf16 ? &ff_gemm_pair<kMode, true, 128> : &ff_gemm_pair<kMode, false, 128>, dim3(grid), kFfThreads,
+                            ff_smem_bytes<128>(), call.stream, p);
+    return launch_dense(name, bf16 ? &ff_gemm_pair<kMode, true, 256> : &ff_gemm_pair<kMode, false, 256>, dim3(grid), kFfThreads,
+                        ff_smem_bytes<256>(), call.stream, p);
+}
+
+constexpr long long kFfNarrowCost = 65;   // a 128-wide tile's time in hundredths of a 256-wide one's (62 to 68 measured)
+// Width of the merged B: 128 where whole rounds of 256-wide tiles over the CTA pairs cost more.  `row_tiles` counts every batch.
+int ff_tile_n(int row_tiles, int cols256, int cols128, int sm_count) {
+    const int pairs = sm_count / 2;
+    const long long wide = (static_cast<long long>(row_tiles) * cols256 + pairs - 1) / pairs;
+    const long long narrow = (static_cast<long long>(row_tiles) * cols128 + pairs - 1) / pairs;
+    return narrow * kFfNarrowCost < wide * 100 ? 128 : 256;
 }
 
 // CTAs that share the k range of one tile: as many as the GPU has room for, with at least four steps each.
@@ -177,22 +192,35 @@ template <FewOp kOp> int launch_few(FewProblem& p, int dtype, DenseCall& call, u
         default: return bf16 ? launch_few_as<kOp, 128, true>(p, call) : launch_few_as<kOp, 128, false>(p, call);
     }
 }
-constexpr int kFewMost = 256;
+// Whether the few-token kernel or the CTA-pair kernel is faster.  Up to 64 rows always the former.  Beyond, its tiles are
+// 128 x 128 and it gains as long as two CTAs or more can share the k range of each.  Measured, few-token against pair:
+//   fp8    m=256: n=4096 k=7168 (64 tiles) 19.8 / 26.7 us, n=7168 k=2048 (112) 13.5 / 11.6; m=128 n=14336 k=4096 (112) 21.7 / 18.9
+//   gated  m=256 n=4096 k=7168 (64) 35.4 / 41.1, but with a short k range, where the exchange counts: m=128 n=7168 k=2048 (56)
+//          19.9 / 17.4, m=1024 n=k=1024 (64) 13.3 / 10.5, m=512 n=k=1024 (32) 10.4 / 10.5
+bool few_is_faster(FewOp op, int m, int n, int steps, int sm_count) {
+    if (m <= 64) return true;
+    const long long tiles = static_cast<long long>((n + 127) / 128) * ((m + 127) / 128);
+    if (2 * tiles > sm_count) return false;
+    return op == FewOp::Few8 || steps >= 64 || 4 * tiles <= sm_count;
+}
 constexpr int kFuseMost = 16;            // rows up to which fp8_linear quantises inside the product's kernel
 
 // Maps and sizes that the forward pass and its recomputation share.
-int ff_projections(FfProblem& p, const void* x, long long ldx, const void* w1, long long ldw1, const void* w2, long long ldw2,
-                   int act, int m, int n, int k) {
+int ff_projections(FfProblem& p, int* tile_n, const void* x, long long ldx, const void* w1, long long ldw1, const void* w2,
+                   long long ldw2, int act, int m, int n, int k, bool keep, int sm_count) {
     int rc;
+    p.m_tiles = (m + 255) / 256;
+    // 8-bit copies are made from whole 128-wide blocks
+    *tile_n = keep ? 256 : ff_tile_n(p.m_tiles, (n + 127) / 128, (n + 63) / 64, sm_count);
+    const int cols = *tile_n / 2;
     if ((rc = encode_matrix_map(&p.a[0], x, 2, k, m, ldx, 64, 128))) return rc;
-    if ((rc = encode_matrix_map(&p.b[0], w1, 2, k, n, ldw1, 64, 128))) return rc;
-    if ((rc = encode_matrix_map(&p.b[1], w2, 2, k, n, ldw2, 64, 128))) return rc;
+    if ((rc = encode_matrix_map(&p.b[0], w1, 2, k, n, ldw1, 64, cols))) return rc;
+    if ((rc = encode_matrix_map(&p.b[1], w2, 2, k, n, ldw2, 64, cols))) return rc;
     p.rows = m;
     p.cols = n;
     p.k_tiles = (k + 63) / 64;
     p.segments = 1;
-    p.m_tiles = (m + 255) / 256;
-    p.n_tiles = (n + 127) / 128;
+    p.n_tiles = (n + cols - 1) / cols;
     p.batches = 1;
     p.gelu = act == B200_ACT_GELU;
     return 0;
@@ -266,7 +294,7 @@ size_t fp8_codes_bytes(int m, int k) { return static_cast<size_t>(m) * ((k + 15)
 int fp8_gemm_launch(const Fp8Matrix& a, const Fp8Matrix& b, void* c, long long ldc, int out_dtype, int m, int n, int k,
                     bool after_quantiser, DenseCall& call, uint32_t* status) {
     int rc;
-    if (m <= kFewMost) {
+    if (few_is_faster(FewOp::Few8, m, n, (k + kFp8Block - 1) / kFp8Block, call.st->sm_count)) {
         FewProblem p;
         memset(&p, 0, sizeof p);
         if ((rc = encode_matrix_map(&p.w[0], b.q, 1, k, n, b.ld, 128, 128))) return rc;
@@ -457,7 +485,7 @@ int b200_gated_forward(const void* x, int64_t ldx, const void* w1, int64_t ldw1,
         return fail(B200_E_WORKSPACE, "%s: the 8-bit copies need %zu bytes, 16-byte aligned", what, b200_gated_kept_bytes(m, n, k, keep_x));
     DenseCall call(device, stream);
     if (call.rc) return call.rc;
-    if (!kept && m <= kFewMost) {
+    if (!kept && few_is_faster(FewOp::FewGated, m, n, (k + 63) / 64, call.st->sm_count)) {
         FewProblem f;
         memset(&f, 0, sizeof f);
         if ((rc = encode_matrix_map(&f.w[0], w1, 2, k, n, ldw1, 64, 128))) return rc;
@@ -473,7 +501,8 @@ int b200_gated_forward(const void* x, int64_t ldx, const void* w1, int64_t ldw1,
     }
     FfProblem p;
     memset(&p, 0, sizeof p);
-    if ((rc = ff_projections(p, x, ldx, w1, ldw1, w2, ldw2, act, m, n, k))) return rc;
+    int tile_n;
+    if ((rc = ff_projections(p, &tile_n, x, ldx, w1, ldw1, w2, ldw2, act, m, n, k, kept != nullptr, call.st->sm_count))) return rc;
     if ((rc = encode_matrix_map(&p.out[0], h, 2, n, m, ldh, 64, 32))) return rc;
     if (kept) {
         const Kept v(kept, m, n, k, keep_x != 0);
@@ -486,7 +515,7 @@ int b200_gated_forward(const void* x, int64_t ldx, const void* w1, int64_t ldw1,
         p.keep = 1;
         if (keep_x && (rc = quantize_rows_launch(what, x, dtype, m, k, ldx, v.qx, v.ldk, v.sx, 1, m, 1, call))) return rc;
     }
-    return launch_ff<FfMode::Forward>("ff_gemm_pair<Forward>", p, dtype, call, status);
+    return launch_ff<FfMode::Forward>("ff_gemm_pair<Forward>", p, tile_n, dtype, call, status);
 }
 
 int b200_gated_backward(const void* x, int64_t ldx, const void* kept, size_t kept_bytes, int keep_x, const void* w1, int64_t ldw1,
@@ -533,12 +562,13 @@ int b200_gated_backward(const void* x, int64_t ldx, const void* kept, size_t kep
     } else {
         FfProblem p;
         memset(&p, 0, sizeof p);
-        if ((rc = ff_projections(p, x, ldx, w1, ldw1, w2, ldw2, act, m, n, k))) return rc;
+        int tile_n;
+        if ((rc = ff_projections(p, &tile_n, x, ldx, w1, ldw1, w2, ldw2, act, m, n, k, false, call.st->sm_count))) return rc;
         if ((rc = encode_matrix_map(&p.out[0], dg, 2, n, m, n, 64, 32))) return rc;
         if ((rc = encode_matrix_map(&p.out[1], du, 2, n, m, n, 64, 32))) return rc;
         p.dh = static_cast<const uint16_t*>(dh);
         p.ld_dh = ld_dh;
-        if ((rc = launch_ff<FfMode::GradHidden>("ff_gemm_pair<GradHidden>", p, dtype, call, status))) return rc;
+        if ((rc = launch_ff<FfMode::GradHidden>("ff_gemm_pair<GradHidden>", p, tile_n, dtype, call, status))) return rc;
     }
     if (dx) {
         FfProblem p;
@@ -553,9 +583,10 @@ int b200_gated_backward(const void* x, int64_t ldx, const void* kept, size_t kep
         p.k_tiles = (n + 63) / 64;
         p.segments = 2;
         p.m_tiles = (m + 255) / 256;
-        p.n_tiles = (k + 255) / 256;
         p.batches = 1;
-        if ((rc = launch_ff<FfMode::GradInput>("ff_gemm_pair<GradInput>", p, dtype, call, status))) return rc;
+        const int tile_n = ff_tile_n(p.m_tiles, (k + 255) / 256, (k + 127) / 128, call.st->sm_count);
+        p.n_tiles = (k + tile_n - 1) / tile_n;
+        if ((rc = launch_ff<FfMode::GradInput>("ff_gemm_pair<GradInput>", p, tile_n, dtype, call, status))) return rc;
     }
     if (weights) {
         FfProblem p;
@@ -574,8 +605,9 @@ int b200_gated_backward(const void* x, int64_t ldx, const void* kept, size_t kep
         p.k_tiles = (m + 63) / 64;
         p.segments = 1;
         p.m_tiles = (n + 255) / 256;
-        p.n_tiles = (k + 255) / 256;
-        if ((rc = launch_ff<FfMode::GradWeight>("ff_gemm_pair<GradWeight>", p, dtype, call, status))) return rc;
+        const int tile_n = ff_tile_n(p.m_tiles * p.batches, (k + 255) / 256, (k + 127) / 128, call.st->sm_count);
+        p.n_tiles = (k + tile_n - 1) / tile_n;
+        if ((rc = launch_ff<FfMode::GradWeight>("ff_gemm_pair<GradWeight>", p, tile_n, dtype, call, status))) return rc;
     }
     return 0;
 }

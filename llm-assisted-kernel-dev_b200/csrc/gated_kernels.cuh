@@ -42,19 +42,26 @@ struct FfProblem {
     uint32_t* status;
 };
 
-constexpr int kFfStages = 5;
-constexpr uint32_t kFfOperandBytes = 128u * 128u;            // 128 rows x 64 k (K-major) or 2 boxes of 64 x 64 (MN-major)
-constexpr uint32_t kFfStageBytes = 2u * kFfOperandBytes;
-constexpr uint32_t kFfStagingBytes = 8u * 8192u;             // per epilogue warp two boxes of 32 rows x 128 bytes
+// Shapes of one pair's tile: the merged B has kN rows, half of them in each CTA.  256 is the full-rate shape.  128 (outputs of
+// 256 x 64 or 256 x 128) takes 0.65 of its time instead of half (the loads bound it), and is taken where 256 leaves pairs idle.
+template <int kN> struct FfShape {
+    static constexpr uint32_t kABytes = 128u * 128u;             // 128 rows x 64 k (K-major) or 2 boxes of 64 x 64 (MN-major)
+    static constexpr uint32_t kBBytes = kN / 2 * 128u;
+    static constexpr uint32_t kStageBytes = kABytes + kBBytes;
+    static constexpr int kStages = kN == 256 ? 5 : 6;
+};
+constexpr uint32_t kFfStagingBytes = 8u * 8192u;                 // per epilogue warp two boxes of 32 rows x 128 bytes
 constexpr int kFfThreads = 320;
 
 struct FfControl {
-    uint64_t full[kFfStages], empty[kFfStages];
+    uint64_t full[6], empty[6];
     uint64_t acc_full[2], acc_release[2], done;
     uint32_t tmem_base, abort_flag;
 };
-constexpr uint32_t kFfSmemBytes = 1024u + kFfStages * kFfStageBytes + kFfStagingBytes + sizeof(FfControl);
-static_assert(kFfSmemBytes <= 227u * 1024u, "shared memory budget");
+template <int kN> constexpr uint32_t ff_smem_bytes() {
+    return 1024u + FfShape<kN>::kStages * FfShape<kN>::kStageBytes + kFfStagingBytes + sizeof(FfControl);
+}
+static_assert(ff_smem_bytes<256>() <= 227u * 1024u && ff_smem_bytes<128>() <= 227u * 1024u, "shared memory budget");
 
 // act(z) and, where asked for, act'(z).  sigma saturates to 0 and 1 without a NaN for finite z.
 struct GateValue { float value, slope; };
@@ -76,14 +83,14 @@ template <bool kSlope> __device__ __forceinline__ GateValue gate(float z, int ge
 }
 
 // h = act(g) u of 32 rows x 64 columns (`acc` and `col`: this warp's half).
-template <bool kBf16>
+template <bool kBf16, int kUp>      // u lies kUp columns behind g
 __device__ __forceinline__ void ff_epilogue_forward(const FfProblem& p, uint32_t acc, BoxWriter& w, int row, int col) {
     const uint32_t box = w.acquire();
 #pragma unroll 1
     for (int c = 0; c < 2; ++c) {
         uint32_t g[32], u[32];
         tc_ld_x32(acc + c * 32, g);
-        tc_ld_x32(acc + 128 + c * 32, u);
+        tc_ld_x32(acc + kUp + c * 32, u);
         tc_wait_ld();
         float f[32];
 #pragma unroll
@@ -125,7 +132,6 @@ __device__ __forceinline__ void ff_epilogue_keep(const FfProblem& p, int which, 
 }
 
 // dg and du of 32 rows x 64 columns from the accumulators and dh (`acc` and `col`: this warp's half).
-template <bool kBf16>
 __device__ __forceinline__ void ff_load_dh(const FfProblem& p, int row, int col, int lane, uint4 (&d)[8]) {
     const int r = row + lane;
     const uint16_t* dh = p.dh + r * p.ld_dh + col;
@@ -133,7 +139,7 @@ __device__ __forceinline__ void ff_load_dh(const FfProblem& p, int row, int col,
     for (int j = 0; j < 8; ++j)
         d[j] = (r < p.rows && col + 8 * j < p.cols) ? *reinterpret_cast<const uint4*>(dh + 8 * j) : make_uint4(0, 0, 0, 0);
 }
-template <bool kBf16>
+template <bool kBf16, int kUp>
 __device__ __forceinline__ void ff_epilogue_grad_hidden(const FfProblem& p, uint32_t acc, BoxWriter& w, int row, int col,
                                                         const uint4 (&d)[8]) {
 #pragma unroll
@@ -143,7 +149,7 @@ __device__ __forceinline__ void ff_epilogue_grad_hidden(const FfProblem& p, uint
         for (int c = 0; c < 4; ++c) {
             uint32_t g[16], u[16];
             tc_ld_x16(acc + c * 16, g);
-            if (which == 0) tc_ld_x16(acc + 128 + c * 16, u);
+            if (which == 0) tc_ld_x16(acc + kUp + c * 16, u);
             tc_wait_ld();
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -165,12 +171,12 @@ __device__ __forceinline__ void ff_epilogue_grad_hidden(const FfProblem& p, uint
     }
 }
 
-// 32 rows x 128 columns of a plain product.
-template <bool kBf16>
+// 32 rows x 64 kParts columns of a plain product.
+template <bool kBf16, int kParts>
 __device__ __forceinline__ void ff_epilogue_plain(const FfProblem& p, const CUtensorMap* map, uint32_t acc, BoxWriter& w,
                                                   int row, int col) {
 #pragma unroll 1
-    for (int part = 0; part < 2; ++part) {
+    for (int part = 0; part < kParts; ++part) {
         const uint32_t box = w.acquire();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -186,24 +192,26 @@ __device__ __forceinline__ void ff_epilogue_plain(const FfProblem& p, const CUte
     }
 }
 
-template <FfMode kMode, bool kBf16>
+template <FfMode kMode, bool kBf16, int kN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfThreads, 1)
 ff_gemm_pair(const __grid_constant__ FfProblem p) {
+    using S = FfShape<kN>;
+    constexpr int kStages = S::kStages;
     constexpr bool kDual = kMode == FfMode::Forward || kMode == FfMode::GradHidden;
     constexpr bool kAMn = kMode == FfMode::GradWeight;
     constexpr bool kBMn = kMode == FfMode::GradWeight || kMode == FfMode::GradInput;
-    constexpr int kTileCols = kDual ? 128 : 256;
+    constexpr int kTileCols = kDual ? kN / 2 : kN;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    FfControl* ctl = reinterpret_cast<FfControl*>(smem_raw + (smem_base - smem_u32(smem_raw)) + kFfStages * kFfStageBytes +
-                                                  kFfStagingBytes);
+    const uint32_t staging = smem_base + kStages * S::kStageBytes;
+    FfControl* ctl = reinterpret_cast<FfControl*>(smem_raw + (staging - smem_u32(smem_raw)) + kFfStagingBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_cta_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int steps = p.k_tiles * p.segments;
     volatile uint32_t* abort_flag = &ctl->abort_flag;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kFfStages; ++s) {
+        for (int s = 0; s < kStages; ++s) {
             mbar_init(smem_u32(&ctl->full[s]), 1);
             mbar_init(smem_u32(&ctl->empty[s]), 1);
         }
@@ -235,7 +243,7 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
         bool ok = true;
         for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, p.batches); ok && t.valid(); t.next()) {
             const int a_row = t.m * 256 + static_cast<int>(rank) * 128;
-            const int b_row = kDual ? t.n * 128 : t.n * 256 + static_cast<int>(rank) * 128;
+            const int b_row = kDual ? t.n * kTileCols : t.n * kN + static_cast<int>(rank) * (kN / 2);
             for (int i = 0; i < steps; ++i) {
                 const int seg = i >= p.k_tiles ? 1 : 0;
                 const int k0 = (i - seg * p.k_tiles) * 64;
@@ -243,9 +251,9 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
                     ok = false;
                     break;
                 }
-                const uint32_t a_dst = smem_base + s * kFfStageBytes, b_dst = a_dst + kFfOperandBytes;
+                const uint32_t a_dst = smem_base + s * S::kStageBytes, b_dst = a_dst + S::kABytes;
                 const uint32_t bar = map_to_cta(smem_u32(&ctl->full[s]), 0);
-                if (rank == 0) mbar_arrive_expect_tx_elect(smem_u32(&ctl->full[s]), 2 * kFfStageBytes);   // both CTAs' bytes
+                if (rank == 0) mbar_arrive_expect_tx_elect(smem_u32(&ctl->full[s]), 2 * S::kStageBytes);   // both CTAs' bytes
                 const CUtensorMap* ma = &p.a[kMode == FfMode::GradWeight ? t.batch : seg];
                 const CUtensorMap* mb = &p.b[kDual ? rank : (kMode == FfMode::GradInput ? seg : 0)];
                 if constexpr (kAMn) {
@@ -256,11 +264,11 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
                 }
                 if constexpr (kBMn) {
                     tma_load_2d_pair_elect(b_dst, mb, bar, b_row, k0);
-                    tma_load_2d_pair_elect(b_dst + 8192, mb, bar, b_row + 64, k0);
+                    if constexpr (kN == 256) tma_load_2d_pair_elect(b_dst + 8192, mb, bar, b_row + 64, k0);
                 } else {
                     tma_load_2d_pair_elect(b_dst, mb, bar, k0, b_row);
                 }
-                if (++s == kFfStages) { s = 0; ph ^= 1u; }
+                if (++s == kStages) { s = 0; ph ^= 1u; }
             }
         }
         if (!ok)
@@ -269,7 +277,7 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
     } else if (warp == 8) {
         // ------------------------------ MMA issuer
         if (rank == 0) {
-            constexpr uint32_t kIdesc = idesc_dense(256, 256, kBf16 ? 1u : 0u, kAMn, kBMn);
+            constexpr uint32_t kIdesc = idesc_dense(256, kN, kBf16 ? 1u : 0u, kAMn, kBMn);
             uint32_t s = 0, ph = 0;
             int it = 0;
             bool ok = true;
@@ -287,13 +295,13 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
                         break;
                     }
                     tc_fence_after_sync();
-                    const uint32_t a = dense_desc_lo<kAMn>(smem_base + s * kFfStageBytes);
-                    const uint32_t b = dense_desc_lo<kBMn>(smem_base + s * kFfStageBytes + kFfOperandBytes);
+                    const uint32_t a = dense_desc_lo<kAMn>(smem_base + s * S::kStageBytes);
+                    const uint32_t b = dense_desc_lo<kBMn>(smem_base + s * S::kStageBytes + S::kABytes);
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         tc_mma_f16_pair(acc, a + j * kDescStepK16<kAMn>, b + j * kDescStepK16<kBMn>, kIdesc, (i > 0 || j > 0) ? 1u : 0u);
                     tc_commit_pair_both_elect(smem_u32(&ctl->empty[s]), 3);
-                    if (++s == kFfStages) { s = 0; ph ^= 1u; }
+                    if (++s == kStages) { s = 0; ph ^= 1u; }
                 }
                 if (ok) tc_commit_pair_both_elect(smem_u32(&ctl->acc_full[it & 1]), 3);
             }
@@ -303,25 +311,32 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
         __syncwarp();
     } else {
         // ------------------------------ epilogue
+        // a box is 64 columns: the 64 of a narrow dual tile are one warp's work per quadrant
+        constexpr int kWarpCols = kTileCols / 2 < 64 ? 64 : kTileCols / 2;
         const int quad = warp & 3, half = warp >> 2;
-        BoxWriter w{smem_base + kFfStages * kFfStageBytes + static_cast<uint32_t>(warp) * 8192u, lane, 0};
+        const bool works = half * kWarpCols < kTileCols;
+        BoxWriter w{staging + static_cast<uint32_t>(warp) * 8192u, lane, 0};
         const uint32_t release = map_to_cta(smem_u32(&ctl->acc_release[0]), 0);
         int it = 0;
         for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, p.batches); t.valid(); t.next(), ++it) {
             const int row = t.m * 256 + static_cast<int>(rank) * 128 + quad * 32;
-            const int col = t.n * kTileCols + half * (kTileCols / 2);
+            const int col = t.n * kTileCols + half * kWarpCols;
             uint4 d[8];
-            if constexpr (kMode == FfMode::GradHidden) ff_load_dh<kBf16>(p, row, col, lane, d);   // arrives while the products are formed
+            if constexpr (kMode == FfMode::GradHidden)
+                if (works) ff_load_dh(p, row, col, lane, d);          // arrives while the products are formed
             if (!mbar_wait_converged(smem_u32(&ctl->acc_full[it & 1]), (it >> 1) & 1, abort_flag, p.status, kStatusDense)) break;
             tc_fence_after_sync();
             const uint32_t acc = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + (it & 1) * 256;
-            if constexpr (kMode == FfMode::Forward) {
-                ff_epilogue_forward<kBf16>(p, acc + half * 64, w, row, col);
-                if (p.keep) ff_epilogue_keep(p, half, acc + half * 128, w, row, t.n * kTileCols);   // g by one half of the warps, u by the other
-            } else if constexpr (kMode == FfMode::GradHidden) {
-                ff_epilogue_grad_hidden<kBf16>(p, acc + half * 64, w, row, col, d);
-            } else {
-                ff_epilogue_plain<kBf16>(p, &p.out[t.batch], acc + half * 128, w, row, col);
+            if (works) {
+                if constexpr (kMode == FfMode::Forward) {
+                    ff_epilogue_forward<kBf16, kTileCols>(p, acc + half * kWarpCols, w, row, col);
+                    if (kN == 256 && p.keep)                          // g by one half of the warps, u by the other
+                        ff_epilogue_keep(p, half, acc + half * 128, w, row, t.n * kTileCols);
+                } else if constexpr (kMode == FfMode::GradHidden) {
+                    ff_epilogue_grad_hidden<kBf16, kTileCols>(p, acc + half * kWarpCols, w, row, col, d);
+                } else {
+                    ff_epilogue_plain<kBf16, kWarpCols / 64>(p, &p.out[t.batch], acc + half * kWarpCols, w, row, col);
+                }
             }
             tc_fence_before_sync();
             __syncwarp();
