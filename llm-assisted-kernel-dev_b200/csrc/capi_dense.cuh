@@ -66,6 +66,8 @@ struct DenseCall {
         if ((rc = opt_in_few_all<FewOp::FewGated>())) return;
         if ((rc = opt_in_few<FewOp::Few8, 16, true>())) return;
         if ((rc = opt_in_ff<FfMode::Forward>())) return;
+        if ((rc = opt_in_smem(ff_forward_keep<false>, ff_smem_bytes<256>()))) return;
+        if ((rc = opt_in_smem(ff_forward_keep<true>, ff_smem_bytes<256>()))) return;
         if ((rc = opt_in_ff<FfMode::GradHidden>())) return;
         if ((rc = opt_in_ff<FfMode::GradInput>())) return;
         if ((rc = opt_in_ff<FfMode::GradWeight>())) return;
@@ -512,8 +514,11 @@ int b200_gated_forward(const void* x, int64_t ldx, const void* w1, int64_t ldw1,
         p.sf[1] = v.su;
         p.sf_row = 1;
         p.sf_col = m;
-        p.keep = 1;
         if (keep_x && (rc = quantize_rows_launch(what, x, dtype, m, k, ldx, v.qx, v.ldk, v.sx, 1, m, 1, call))) return rc;
+        p.status = status ? status : call.st->status;
+        auto* kernel = dtype == B200_DTYPE_BF16 ? &ff_forward_keep<true> : &ff_forward_keep<false>;
+        return launch_dense("ff_forward_keep", kernel, dim3(pair_grid(static_cast<long long>(p.m_tiles) * p.n_tiles, call.st->sm_count)),
+                            kKeepThreads, ff_smem_bytes<256>(), call.stream, p);
     }
     return launch_ff<FfMode::Forward>("ff_gemm_pair<Forward>", p, tile_n, dtype, call, status);
 }

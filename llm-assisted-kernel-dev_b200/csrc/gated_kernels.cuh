@@ -38,7 +38,7 @@ struct FfProblem {
     int rows, cols;              // of the outputs
     int k_tiles, segments;       // 64-wide steps per segment; segments share the accumulators
     int m_tiles, n_tiles, batches;
-    int gelu, keep;
+    int gelu;
     uint32_t* status;
 };
 
@@ -98,37 +98,6 @@ __device__ __forceinline__ void ff_epilogue_forward(const FfProblem& p, uint32_t
         put_chunk<kBf16>(w, box, c * 4, f);
     }
     w.send(box, &p.out[0], col, row, row < p.rows && col < p.cols);
-}
-
-// 8-bit copy of one projection's 32 rows x 128 columns (a lane holds a whole block: its row's 128 columns).
-__device__ __forceinline__ void ff_epilogue_keep(const FfProblem& p, int which, uint32_t acc, BoxWriter& w, int row, int col) {
-    float m = kAmaxFloor;
-#pragma unroll 1
-    for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        tc_ld_x32(acc + c * 32, v);
-        tc_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) m = fmaxf(m, fabsf(__uint_as_float(v[i])));
-    }
-    const PowerScale s(m);
-    const uint32_t box = w.acquire();
-#pragma unroll 1
-    for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        tc_ld_x32(acc + c * 32, v);
-        tc_wait_ld();
-        uint32_t q[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            q[i] = pack_e4m3x4(s(__uint_as_float(v[4 * i])), s(__uint_as_float(v[4 * i + 1])),
-                               s(__uint_as_float(v[4 * i + 2])), s(__uint_as_float(v[4 * i + 3])));
-        w.put(box, 2 * c, q[0], q[1], q[2], q[3]);
-        w.put(box, 2 * c + 1, q[4], q[5], q[6], q[7]);
-    }
-    w.send(box, &p.kept[which], col, row, row < p.rows && col < p.cols);
-    const int r = row + w.lane;
-    if (r < p.rows && col < p.cols) p.sf[which][r * p.sf_row + (col / kFp8Block) * p.sf_col] = s.scale;
 }
 
 // dg and du of 32 rows x 64 columns from the accumulators and dh (`acc` and `col`: this warp's half).
@@ -192,6 +161,134 @@ __device__ __forceinline__ void ff_epilogue_plain(const FfProblem& p, const CUte
     }
 }
 
+// Producer warp: this CTA's rows of A and its half of B, step after step.
+template <FfMode kMode, int kN>
+__device__ __forceinline__ void ff_produce(const FfProblem& p, FfControl* ctl, uint32_t smem_base, uint32_t rank, int pair, int pairs) {
+    using S = FfShape<kN>;
+    constexpr bool kDual = kMode == FfMode::Forward || kMode == FfMode::GradHidden;
+    constexpr bool kAMn = kMode == FfMode::GradWeight, kBMn = kAMn || kMode == FfMode::GradInput;
+    volatile uint32_t* abort_flag = &ctl->abort_flag;
+    const int steps = p.k_tiles * p.segments;
+    uint32_t s = 0, ph = 0;
+    bool ok = true;
+    for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, p.batches); ok && t.valid(); t.next()) {
+        const int a_row = t.m * 256 + static_cast<int>(rank) * 128;
+        const int b_row = kDual ? t.n * (kN / 2) : t.n * kN + static_cast<int>(rank) * (kN / 2);
+        for (int i = 0; i < steps; ++i) {
+            const int seg = i >= p.k_tiles ? 1 : 0;
+            const int k0 = (i - seg * p.k_tiles) * 64;
+            ok = mbar_wait_converged(smem_u32(&ctl->empty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense);
+            if (!ok) break;
+            const uint32_t a_dst = smem_base + s * S::kStageBytes, b_dst = a_dst + S::kABytes;
+            const uint32_t bar = map_to_cta(smem_u32(&ctl->full[s]), 0);
+            if (rank == 0) mbar_arrive_expect_tx_elect(smem_u32(&ctl->full[s]), 2 * S::kStageBytes);   // both CTAs' bytes
+            const CUtensorMap* ma = &p.a[kMode == FfMode::GradWeight ? t.batch : seg];
+            const CUtensorMap* mb = &p.b[kDual ? rank : (kMode == FfMode::GradInput ? seg : 0)];
+            if constexpr (kAMn) {
+                tma_load_2d_pair_elect(a_dst, ma, bar, a_row, k0);
+                tma_load_2d_pair_elect(a_dst + 8192, ma, bar, a_row + 64, k0);
+            } else {
+                tma_load_2d_pair_elect(a_dst, ma, bar, k0, a_row);
+            }
+            if constexpr (kBMn) {
+                tma_load_2d_pair_elect(b_dst, mb, bar, b_row, k0);
+                if constexpr (kN == 256) tma_load_2d_pair_elect(b_dst + 8192, mb, bar, b_row + 64, k0);
+            } else {
+                tma_load_2d_pair_elect(b_dst, mb, bar, k0, b_row);
+            }
+            if (++s == S::kStages) { s = 0; ph ^= 1u; }
+        }
+    }
+    if (!ok)
+        for (int i = 0; i < 64; ++i) __nanosleep(2000);   // error path: let copies in flight land
+    __syncwarp();
+}
+
+// MMA warp (the pair's first CTA issues): `chunk` steps go into one accumulator, then the other one is used.
+template <FfMode kMode, bool kBf16, int kN>
+__device__ __forceinline__ void ff_issue(const FfProblem& p, FfControl* ctl, uint32_t smem_base, uint32_t tmem_base, uint32_t rank,
+                                         int pair, int pairs, int chunk) {
+    using S = FfShape<kN>;
+    constexpr bool kAMn = kMode == FfMode::GradWeight, kBMn = kAMn || kMode == FfMode::GradInput;
+    constexpr uint32_t kIdesc = idesc_dense(256, kN, kBf16 ? 1u : 0u, kAMn, kBMn);
+    volatile uint32_t* abort_flag = &ctl->abort_flag;
+    if (rank == 0) {
+        const int steps = p.k_tiles * p.segments;
+        uint32_t s = 0, ph = 0;
+        int it = 0;
+        bool ok = true;
+        for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, p.batches); ok && t.valid(); t.next()) {
+            for (int i0 = 0; ok && i0 < steps; i0 += chunk, ++it) {
+                if (it >= 2)
+                    ok = mbar_wait_converged(smem_u32(&ctl->acc_release[it & 1]), ((it >> 1) - 1) & 1, abort_flag, p.status, kStatusDense);
+                if (!ok) break;
+                tc_fence_after_sync();
+                const uint32_t acc = tmem_base + (it & 1) * 256;
+                const int count = steps - i0 < chunk ? steps - i0 : chunk;
+#pragma unroll 1
+                for (int i = 0; i < count; ++i) {
+                    ok = mbar_wait_converged(smem_u32(&ctl->full[s]), ph, abort_flag, p.status, kStatusDense);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    const uint32_t a = dense_desc_lo<kAMn>(smem_base + s * S::kStageBytes);
+                    const uint32_t b = dense_desc_lo<kBMn>(smem_base + s * S::kStageBytes + S::kABytes);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        tc_mma_f16_pair(acc, a + j * kDescStepK16<kAMn>, b + j * kDescStepK16<kBMn>, kIdesc, (i > 0 || j > 0) ? 1u : 0u);
+                    tc_commit_pair_both_elect(smem_u32(&ctl->empty[s]), 3);
+                    if (++s == S::kStages) { s = 0; ph ^= 1u; }
+                }
+                if (ok) tc_commit_pair_both_elect(smem_u32(&ctl->acc_full[it & 1]), 3);
+            }
+        }
+        tc_commit_pair_elect(smem_u32(&ctl->done));
+        mbar_wait<true>(smem_u32(&ctl->done), 0, abort_flag, p.status, kStatusDense);
+    }
+    __syncwarp();
+}
+
+// Barriers and tensor memory of a pair's CTA; returns the tensor memory's base.  `alloc_warp` allocates.
+template <int kStages>
+__device__ __forceinline__ uint32_t ff_setup(FfControl* ctl, int warp, int alloc_warp) {
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(smem_u32(&ctl->full[s]), 1);
+            mbar_init(smem_u32(&ctl->empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&ctl->acc_full[b]), 1);
+            mbar_init(smem_u32(&ctl->acc_release[b]), 16);   // eight epilogue warps of each CTA; used in the first
+        }
+        mbar_init(smem_u32(&ctl->done), 1);
+        ctl->abort_flag = 0;
+        fence_mbar_init();
+        fence_proxy_async_smem();
+    }
+    if (warp == alloc_warp) {
+        tmem_alloc_pair(smem_u32(&ctl->tmem_base), 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    cluster_arrive();
+    cluster_wait();            // both CTAs' barriers exist
+    griddep_launch_dependents();   // after this CTA has its tensor memory: a CTA of the next kernel cannot take it away
+    griddep_wait();
+    return ctl->tmem_base;
+}
+// Nobody leaves while the partner may still signal its barriers or while MMAs run on this SM.
+__device__ __forceinline__ void ff_leave(uint32_t tmem_base, int warp, int alloc_warp) {
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    if (warp == alloc_warp) {
+        tc_fence_after_sync();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
 template <FfMode kMode, bool kBf16, int kN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfThreads, 1)
 ff_gemm_pair(const __grid_constant__ FfProblem p) {
@@ -208,108 +305,11 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_cta_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-    const int steps = p.k_tiles * p.segments;
     volatile uint32_t* abort_flag = &ctl->abort_flag;
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
-            mbar_init(smem_u32(&ctl->full[s]), 1);
-            mbar_init(smem_u32(&ctl->empty[s]), 1);
-        }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(smem_u32(&ctl->acc_full[b]), 1);
-            mbar_init(smem_u32(&ctl->acc_release[b]), 16);   // eight epilogue warps of each CTA; used in the first
-        }
-        mbar_init(smem_u32(&ctl->done), 1);
-        ctl->abort_flag = 0;
-        fence_mbar_init();
-        fence_proxy_async_smem();
-    }
-    if (warp == 8) {
-        tmem_alloc_pair(smem_u32(&ctl->tmem_base), 512);
-        tmem_relinquish_pair();
-    }
-    tc_fence_before_sync();
-    __syncthreads();
-    tc_fence_after_sync();
-    cluster_arrive();
-    cluster_wait();            // both CTAs' barriers exist
-    const uint32_t tmem_base = ctl->tmem_base;
-    griddep_launch_dependents();   // after this CTA has its tensor memory: a CTA of the next kernel cannot take it away
-    griddep_wait();
-
-    if (warp == 9) {
-        // ------------------------------ producer: this CTA's rows of A and its half of B
-        uint32_t s = 0, ph = 0;
-        bool ok = true;
-        for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, p.batches); ok && t.valid(); t.next()) {
-            const int a_row = t.m * 256 + static_cast<int>(rank) * 128;
-            const int b_row = kDual ? t.n * kTileCols : t.n * kN + static_cast<int>(rank) * (kN / 2);
-            for (int i = 0; i < steps; ++i) {
-                const int seg = i >= p.k_tiles ? 1 : 0;
-                const int k0 = (i - seg * p.k_tiles) * 64;
-                if (!__all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->empty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense))) {
-                    ok = false;
-                    break;
-                }
-                const uint32_t a_dst = smem_base + s * S::kStageBytes, b_dst = a_dst + S::kABytes;
-                const uint32_t bar = map_to_cta(smem_u32(&ctl->full[s]), 0);
-                if (rank == 0) mbar_arrive_expect_tx_elect(smem_u32(&ctl->full[s]), 2 * S::kStageBytes);   // both CTAs' bytes
-                const CUtensorMap* ma = &p.a[kMode == FfMode::GradWeight ? t.batch : seg];
-                const CUtensorMap* mb = &p.b[kDual ? rank : (kMode == FfMode::GradInput ? seg : 0)];
-                if constexpr (kAMn) {
-                    tma_load_2d_pair_elect(a_dst, ma, bar, a_row, k0);
-                    tma_load_2d_pair_elect(a_dst + 8192, ma, bar, a_row + 64, k0);
-                } else {
-                    tma_load_2d_pair_elect(a_dst, ma, bar, k0, a_row);
-                }
-                if constexpr (kBMn) {
-                    tma_load_2d_pair_elect(b_dst, mb, bar, b_row, k0);
-                    if constexpr (kN == 256) tma_load_2d_pair_elect(b_dst + 8192, mb, bar, b_row + 64, k0);
-                } else {
-                    tma_load_2d_pair_elect(b_dst, mb, bar, k0, b_row);
-                }
-                if (++s == kStages) { s = 0; ph ^= 1u; }
-            }
-        }
-        if (!ok)
-            for (int i = 0; i < 64; ++i) __nanosleep(2000);   // error path: let copies in flight land
-        __syncwarp();
-    } else if (warp == 8) {
-        // ------------------------------ MMA issuer
-        if (rank == 0) {
-            constexpr uint32_t kIdesc = idesc_dense(256, kN, kBf16 ? 1u : 0u, kAMn, kBMn);
-            uint32_t s = 0, ph = 0;
-            int it = 0;
-            bool ok = true;
-            for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, p.batches); ok && t.valid(); t.next(), ++it) {
-                if (it >= 2)
-                    ok = __all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->acc_release[it & 1]), ((it >> 1) - 1) & 1, abort_flag,
-                                                           p.status, kStatusDense));
-                if (!ok) break;
-                tc_fence_after_sync();
-                const uint32_t acc = tmem_base + (it & 1) * 256;
-#pragma unroll 1
-                for (int i = 0; i < steps; ++i) {
-                    if (!__all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->full[s]), ph, abort_flag, p.status, kStatusDense))) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after_sync();
-                    const uint32_t a = dense_desc_lo<kAMn>(smem_base + s * S::kStageBytes);
-                    const uint32_t b = dense_desc_lo<kBMn>(smem_base + s * S::kStageBytes + S::kABytes);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        tc_mma_f16_pair(acc, a + j * kDescStepK16<kAMn>, b + j * kDescStepK16<kBMn>, kIdesc, (i > 0 || j > 0) ? 1u : 0u);
-                    tc_commit_pair_both_elect(smem_u32(&ctl->empty[s]), 3);
-                    if (++s == kStages) { s = 0; ph ^= 1u; }
-                }
-                if (ok) tc_commit_pair_both_elect(smem_u32(&ctl->acc_full[it & 1]), 3);
-            }
-            tc_commit_pair_elect(smem_u32(&ctl->done));
-            mbar_wait<true>(smem_u32(&ctl->done), 0, abort_flag, p.status, kStatusDense);
-        }
-        __syncwarp();
-    } else {
+    const uint32_t tmem_base = ff_setup<S::kStages>(ctl, warp, 8);
+    if (warp == 9) ff_produce<kMode, kN>(p, ctl, smem_base, rank, pair, pairs);
+    else if (warp == 8) ff_issue<kMode, kBf16, kN>(p, ctl, smem_base, tmem_base, rank, pair, pairs, p.k_tiles * p.segments);
+    else {
         // ------------------------------ epilogue
         // a box is 64 columns: the 64 of a narrow dual tile are one warp's work per quadrant
         constexpr int kWarpCols = kTileCols / 2 < 64 ? 64 : kTileCols / 2;
@@ -330,8 +330,6 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
             if (works) {
                 if constexpr (kMode == FfMode::Forward) {
                     ff_epilogue_forward<kBf16, kTileCols>(p, acc + half * kWarpCols, w, row, col);
-                    if (kN == 256 && p.keep)                          // g by one half of the warps, u by the other
-                        ff_epilogue_keep(p, half, acc + half * 128, w, row, t.n * kTileCols);
                 } else if constexpr (kMode == FfMode::GradHidden) {
                     ff_epilogue_grad_hidden<kBf16, kTileCols>(p, acc + half * kWarpCols, w, row, col, d);
                 } else {
@@ -345,15 +343,152 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
         if (lane == 0) bulk_wait_group_read_all();
         __syncwarp();
     }
-    // Nobody leaves while the partner may still signal its barriers or while MMAs run on this SM.
-    tc_fence_before_sync();
-    __syncthreads();
-    cluster_arrive();
-    cluster_wait();
-    if (warp == 8) {
-        tc_fence_after_sync();
-        tmem_dealloc_pair(tmem_base, 512);
+    ff_leave(tmem_base, warp, 8);
+}
+
+// The forward pass that also makes the 8-bit copies of g and u.  Tensor memory adds with truncation, one MMA after the other:
+// over a k range of 7168 that left one code in 3400 the neighbour of the right one, 6 to 12 % away, and made the gradients
+// of the weights 1.53 times as far off as their own rounding alone.  So the accumulators are emptied every
+// kKeepChunk steps into fp32 registers (the two accumulators take turns, the MMAs do not wait): one code in XXXX, 1.43 times, and no slower.
+// Each of the eight epilogue warps sums 32 rows x 64 columns of g and of u; the two warps of a quadrant agree on a row's largest
+// magnitudes through shared memory.  Registers: 384 threads start with 168; the two epilogue warpgroups take 216, the third keeps 72.
+constexpr int kKeepThreads = 384, kKeepChunk = 16;
+constexpr uint32_t kKeepSumRegs = 216, kKeepOtherRegs = 72;
+static_assert(256 * kKeepSumRegs + 128 * kKeepOtherRegs <= kKeepThreads * 168, "register split");
+
+// Barrier of the two warps of a quadrant; the second form also tells both whether both are well, so that neither waits for a
+// partner that has given up.
+__device__ __forceinline__ void quad_bar_sync(int quad) { asm volatile("bar.sync %0, 64;" ::"r"(quad + 1) : "memory"); }
+__device__ __forceinline__ bool quad_bar_and(int quad, bool ok) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %2, 0;\n\t"
+        "bar.red.and.pred q, %1, 64, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t"
+        "}\n"
+        : "=r"(all)
+        : "r"(quad + 1), "r"(static_cast<uint32_t>(ok))
+        : "memory");
+    return all != 0;
+}
+
+template <bool kBf16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kKeepThreads, 1)
+ff_forward_keep(const __grid_constant__ FfProblem p) {
+    using S = FfShape<256>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t staging = smem_base + S::kStages * S::kStageBytes;
+    FfControl* ctl = reinterpret_cast<FfControl*>(smem_raw + (staging - smem_u32(smem_raw)) + kFfStagingBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_cta_rank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    volatile uint32_t* abort_flag = &ctl->abort_flag;
+    const uint32_t tmem_base = ff_setup<S::kStages>(ctl, warp, 8);
+    if (warp >= 8) {
+        warpgroup_reg_dec<kKeepOtherRegs>();
+        if (warp == 9) ff_produce<FfMode::Forward, 256>(p, ctl, smem_base, rank, pair, pairs);
+        else if (warp == 8) ff_issue<FfMode::Forward, kBf16, 256>(p, ctl, smem_base, tmem_base, rank, pair, pairs, kKeepChunk);
+    } else {
+        warpgroup_reg_inc<kKeepSumRegs>();
+        const int quad = warp & 3, half = warp >> 2;
+        // one box per warp for h; one for the codes of g and one for those of u per quadrant
+        const uint32_t box_h = staging + static_cast<uint32_t>(warp) * 4096u;
+        const uint32_t box_q = staging + 8u * 4096u + static_cast<uint32_t>(quad) * 8192u;
+        const uint32_t release = map_to_cta(smem_u32(&ctl->acc_release[0]), 0);
+        const uint32_t own = static_cast<uint32_t>(lane) * 128u, swz = static_cast<uint32_t>(lane & 7);
+        const int chunks = (p.k_tiles + kKeepChunk - 1) / kKeepChunk;
+        int it = 0;
+        bool ok = true;
+        for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, 1); ok && t.valid(); t.next()) {
+            uint64_t g[32], u[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) g[i] = u[i] = 0;
+#pragma unroll 1
+            for (int c = 0; c < chunks; ++c, ++it) {
+                ok = mbar_wait_converged(smem_u32(&ctl->acc_full[it & 1]), (it >> 1) & 1, abort_flag, p.status, kStatusDense);
+                if (!ok) break;
+                tc_fence_after_sync();
+                const uint32_t acc = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + (it & 1) * 256 + half * 64;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t v[16];
+                    tc_ld_x16(acc + j * 16, v);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) g[j * 8 + i] = add_f32x2(g[j * 8 + i], pack_f32x2(v[2 * i], v[2 * i + 1]));
+                    tc_ld_x16(acc + 128 + j * 16, v);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) u[j * 8 + i] = add_f32x2(u[j * 8 + i], pack_f32x2(v[2 * i], v[2 * i + 1]));
+                }
+                tc_fence_before_sync();
+                mbar_arrive_cluster_relaxed_elect(release + 8 * (it & 1));
+            }
+            const int row = t.m * 256 + static_cast<int>(rank) * 128 + quad * 32, col = t.n * 128;
+            // boxes and scratch are free once the previous tile's copies have been read
+            if (lane == 0) bulk_wait_group_read_all();
+            __syncwarp();
+            ok = quad_bar_and(quad, ok);
+            if (!ok) break;
+            float mg = kAmaxFloor, mu = kAmaxFloor;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 a = unpack_f32x2(g[j * 4 + i]), b = unpack_f32x2(u[j * 4 + i]);
+                    mg = fmaxf(mg, fmaxf(fabsf(a.x), fabsf(a.y)));
+                    mu = fmaxf(mu, fmaxf(fabsf(b.x), fabsf(b.y)));
+                    w[i] = pack_16<kBf16>(gate<false>(a.x, p.gelu).value * b.x, gate<false>(a.y, p.gelu).value * b.y);
+                }
+                st_shared_v4(box_h + own + ((static_cast<uint32_t>(j) ^ swz) << 4), w[0], w[1], w[2], w[3]);
+            }
+            // largest magnitudes of the whole 128-wide block: the partner warp has the other half
+            const uint32_t scratch = box_q + static_cast<uint32_t>(lane) * 16u;
+            st_shared_f32(scratch + half * 8, mg);
+            st_shared_f32(scratch + half * 8 + 4, mu);
+            quad_bar_sync(quad);
+            uint32_t om, ou;
+            ld_shared_v2(scratch + (half ^ 1) * 8, om, ou);
+            mg = fmaxf(mg, __uint_as_float(om));
+            mu = fmaxf(mu, __uint_as_float(ou));
+            quad_bar_sync(quad);                     // read before the codes take its place
+            const PowerScale sg(mg), su(mu);
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                const PowerScale& sc = which ? su : sg;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t q[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 a = unpack_f32x2((which ? u : g)[j * 8 + 2 * i]), b = unpack_f32x2((which ? u : g)[j * 8 + 2 * i + 1]);
+                        q[i] = pack_e4m3x4(sc(a.x), sc(a.y), sc(b.x), sc(b.y));
+                    }
+                    st_shared_v4(box_q + which * 4096u + own + ((static_cast<uint32_t>(half * 4 + j) ^ swz) << 4), q[0], q[1], q[2], q[3]);
+                }
+            }
+            if (half == 0 && row + lane < p.rows && col < p.cols) {
+                const long long at = (row + lane) * p.sf_row + (col / kFp8Block) * p.sf_col;
+                p.sf[0][at] = sg.scale;
+                p.sf[1][at] = su.scale;
+            }
+            fence_proxy_async_smem();
+            quad_bar_sync(quad);
+            if (lane == 0) {
+                const bool inside = row < p.rows;
+                if (inside && col + half * 64 < p.cols) tma_store_2d(&p.out[0], box_h, col + half * 64, row);
+                if (inside && col < p.cols) tma_store_2d(&p.kept[half], box_q + half * 4096u, col, row);
+                bulk_commit_group();
+            }
+        }
+        if (lane == 0) bulk_wait_group_read_all();
+        __syncwarp();
     }
+    ff_leave(tmem_base, warp, 8);
 }
 
 // dg and du from the 8-bit copies of g and u: a streaming pass, 2 bytes of codes, 2 of dh and 4 of results per

@@ -219,6 +219,11 @@ __device__ __forceinline__ float2 unpack_e4m3x2(uint32_t v) {
 __device__ __forceinline__ void fma_f32x2(uint64_t& acc, uint64_t x, uint64_t s) {
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(x), "l"(s));
 }
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
 __device__ __forceinline__ uint64_t mul_f32x2(uint64_t x, uint64_t y) {
     uint64_t r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
