@@ -124,7 +124,8 @@ def raise_on_status(device: int, stream: int = 0) -> None:
     word = read_status(device, stream)
     if word:
         raise B200Error(word, f"device status word {word:#x}: an on-device wait ran out (bits: 1 producer, 2/4 MMA, "
-                              f"8 epilogue, 0x10 serial, 0x20 split-k, 0x40 scale factors, 0x80 CTA pair)")
+                              f"8 epilogue, 0x10 serial, 0x20 split-k, 0x40 scale factors, 0x80 CTA pair, "
+                              f"0x100 fp8 and gated kernels)")
 
 
 def last_launch_cycles(device: int, stream: int = 0) -> int:

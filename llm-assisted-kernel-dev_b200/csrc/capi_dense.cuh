@@ -45,6 +45,25 @@ template <FewOp kOp> int opt_in_few_all() {
     return opt_in_few<kOp, 128>();
 }
 
+template <typename K> int load_kernel(K kernel) {
+    cudaFuncAttributes attr;
+    B200_CUDA(cudaFuncGetAttributes(&attr, kernel));
+    return 0;
+}
+// Kernels without a shared-memory opt-in are loaded here rather than by their first launch, which may be captured.
+int load_streaming() {
+    int rc;
+    if ((rc = load_kernel(fp8_quantize_rows<true, true, true>)) || (rc = load_kernel(fp8_quantize_rows<true, true, false>)) ||
+        (rc = load_kernel(fp8_quantize_rows<true, false, true>)) || (rc = load_kernel(fp8_quantize_rows<true, false, false>)) ||
+        (rc = load_kernel(fp8_quantize_rows<false, true, true>)) || (rc = load_kernel(fp8_quantize_rows<false, true, false>)) ||
+        (rc = load_kernel(fp8_quantize_rows<false, false, true>)) || (rc = load_kernel(fp8_quantize_rows<false, false, false>)) ||
+        (rc = load_kernel(fp8_quantize_blocks<true, true>)) || (rc = load_kernel(fp8_quantize_blocks<true, false>)) ||
+        (rc = load_kernel(fp8_quantize_blocks<false, true>)) || (rc = load_kernel(fp8_quantize_blocks<false, false>)) ||
+        (rc = load_kernel(fp8_dequantize_rows<true>)) || (rc = load_kernel(fp8_dequantize_rows<false>)) ||
+        (rc = load_kernel(gated_grad_kept<true>)) || (rc = load_kernel(gated_grad_kept<false>))) return rc;
+    return 0;
+}
+
 // Lock, current device and per-device state of one call.
 struct DenseCall {
     std::lock_guard<std::mutex> lock;
@@ -57,9 +76,9 @@ struct DenseCall {
         // a thread that has not used CUDA yet (autograd runs backward passes on its own threads) has the device but
         // no context, which the tensor-map encoder asks for: cudaSetDevice makes the device's context current
         if ((rc = bind(device))) return;
-        if ((rc = device_state(device, &st))) return;
         bool& ready = g_dense_ready[device];
-        if (ready) return;
+        if (!ready && (rc = reject_first_capture())) return;
+        if ((rc = device_state(device, &st)) || ready) return;
         if ((rc = opt_in_smem(fp8_gemm_pair<false>, kFp8SmemBytes))) return;
         if ((rc = opt_in_smem(fp8_gemm_pair<true>, kFp8SmemBytes))) return;
         if ((rc = opt_in_few_all<FewOp::Few8>())) return;
@@ -71,7 +90,16 @@ struct DenseCall {
         if ((rc = opt_in_ff<FfMode::GradHidden>())) return;
         if ((rc = opt_in_ff<FfMode::GradInput>())) return;
         if ((rc = opt_in_ff<FfMode::GradWeight>())) return;
+        if ((rc = load_streaming())) return;
         ready = true;
+    }
+    // The one-time set-up of a device loads code and clears state, which a capture does not allow.
+    int reject_first_capture() {
+        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+        B200_CUDA(cudaStreamIsCapturing(stream, &cs));
+        if (cs == cudaStreamCaptureStatusNone) return 0;
+        return fail(B200_E_CAPTURE, "the stream is being captured and this is the first call on its device: make one call outside "
+                                    "the capture first");
     }
     static int bind(int device) {
         B200_CUDA(cudaSetDevice(device));

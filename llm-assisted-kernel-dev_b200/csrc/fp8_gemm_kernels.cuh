@@ -93,100 +93,100 @@ fp8_gemm_pair(const __grid_constant__ Fp8Problem p) {
     griddep_wait();
 
     if (warp >= 8) {
-      warpgroup_reg_dec<kFp8OtherRegs>();
-      if (warp == 9) {
-        // ------------------------------ producer: this CTA's 128 rows of A and of B
-        uint32_t s = 0, ph = 0;
-        bool ok = true;
-        for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, 1); ok && t.valid(); t.next()) {
-            const int a_row = t.m * 256 + static_cast<int>(rank) * 128, b_row = t.n * 256 + static_cast<int>(rank) * 128;
-            for (int i = 0; i < p.k_tiles; ++i) {
-                if (!__all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->empty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense))) {
-                    ok = false;
-                    break;
-                }
-                const uint32_t dst = smem_base + s * kFp8StageBytes;
-                const uint32_t bar = map_to_cta(smem_u32(&ctl->full[s]), 0);
-                if (rank == 0) mbar_arrive_expect_tx_elect(smem_u32(&ctl->full[s]), 2 * kFp8StageBytes);   // both CTAs' bytes
-                tma_load_2d_pair_elect(dst, &p.a, bar, i * 128, a_row);
-                tma_load_2d_pair_elect(dst + kFp8OperandBytes, &p.b, bar, i * 128, b_row);
-                if (++s == kFp8Stages) { s = 0; ph ^= 1u; }
-            }
-        }
-        if (!ok)
-            for (int i = 0; i < 64; ++i) __nanosleep(2000);   // error path: let copies in flight land
-        __syncwarp();
-      } else if (warp == 10) {
-        // ------------------------------ scales: products s_A s_B of this CTA's 128 rows and both column halves
-        const uint32_t ring = smem_base + kFp8Stages * kFp8StageBytes + kFp8StagingBytes;
-        uint32_t batch = 0, nth = 0;
-        bool ok = true;
-        for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, 1); ok && t.valid(); t.next(), ++nth) {
-            const int row0 = t.m * 256 + static_cast<int>(rank) * 128, col = t.n * 256;
-            // rows and columns past the matrix get scales that exist; what they scale is never stored
-            const float* sa[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) sa[r] = p.sfa + (row0 + r * 32 + lane < p.m ? row0 + r * 32 + lane : 0) * p.sfa_row;
-            const float* sb = p.sfb + (col / kFp8Block) * p.sfb_row;
-            const long long next_half = col + 128 < p.n ? p.sfb_row : 0;
-            for (int i0 = 0; i0 < p.k_tiles; i0 += kFp8Batch, ++batch) {
-                ok = mbar_wait_converged(smem_u32(&ctl->scale_free[batch & 1]), ((batch >> 1) & 1) ^ 1u, abort_flag, p.status, kStatusDense);
-                if (!ok) break;
-                if (i0 == 0 && lane == 0) ctl->place[nth & 3] = make_int2(row0, col);
-                const uint32_t dst = ring + (batch & 1) * kFp8BatchBytes + lane * 4;
-#pragma unroll
-                for (int part = 0; part < kFp8Batch; part += 4) {
-                    float a[4][4], b[4][2];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int at = i0 + part + j < p.k_tiles ? i0 + part + j : p.k_tiles - 1;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) a[j][r] = sa[r][at * p.sfa_col];
-                        b[j][0] = sb[at * p.sfb_col];
-                        b[j][1] = sb[at * p.sfb_col + next_half];
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            st_shared_f32(dst + (part + j) * 1024 + r * 128, a[j][r] * b[j][0]);
-                            st_shared_f32(dst + (part + j) * 1024 + 512 + r * 128, a[j][r] * b[j][1]);
-                        }
-                }
-                mbar_arrive(smem_u32(&ctl->scale_full[batch & 1]));
-            }
-        }
-        __syncwarp();
-      } else if (warp == 8) {
-        // ------------------------------ MMA issuer
-        if (rank == 0) {
-            constexpr uint32_t kIdesc = idesc_dense(256, 256, 0u, false, false);
-            uint32_t s = 0, ph = 0, cnt = 0;
+        warpgroup_reg_dec<kFp8OtherRegs>();
+        if (warp == 9) {
+            // ------------------------------ producer: this CTA's 128 rows of A and of B
+            uint32_t s = 0, ph = 0;
             bool ok = true;
             for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, 1); ok && t.valid(); t.next()) {
-#pragma unroll 1
-                for (int i = 0; i < p.k_tiles; ++i, ++cnt) {
-                    ok = mbar_wait_converged(smem_u32(&ctl->full[s]), ph, abort_flag, p.status, kStatusDense);
-                    if (ok && cnt >= 2)
-                        ok = mbar_wait_converged(smem_u32(&ctl->acc_release[cnt & 1]), ((cnt >> 1) - 1) & 1, abort_flag, p.status,
-                                                 kStatusDense);
-                    if (!ok) break;
-                    tc_fence_after_sync();
-                    const uint32_t a = dense_desc_lo<false>(smem_base + s * kFp8StageBytes);
-                    const uint32_t acc = tmem_base + (cnt & 1) * 256;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)     // 32 e4m3 elements of k = 32 bytes each
-                        tc_mma_f8_pair(acc, a + 2 * j, a + (kFp8OperandBytes >> 4) + 2 * j, kIdesc, j > 0 ? 1u : 0u);
-                    tc_commit_pair_both_elect(smem_u32(&ctl->acc_full[cnt & 1]), 3);
-                    tc_commit_pair_both_elect(smem_u32(&ctl->empty[s]), 3);
+                const int a_row = t.m * 256 + static_cast<int>(rank) * 128, b_row = t.n * 256 + static_cast<int>(rank) * 128;
+                for (int i = 0; i < p.k_tiles; ++i) {
+                    if (!__all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl->empty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense))) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t dst = smem_base + s * kFp8StageBytes;
+                    const uint32_t bar = map_to_cta(smem_u32(&ctl->full[s]), 0);
+                    if (rank == 0) mbar_arrive_expect_tx_elect(smem_u32(&ctl->full[s]), 2 * kFp8StageBytes);   // both CTAs' bytes
+                    tma_load_2d_pair_elect(dst, &p.a, bar, i * 128, a_row);
+                    tma_load_2d_pair_elect(dst + kFp8OperandBytes, &p.b, bar, i * 128, b_row);
                     if (++s == kFp8Stages) { s = 0; ph ^= 1u; }
                 }
             }
-            tc_commit_pair_elect(smem_u32(&ctl->done));
-            mbar_wait<true>(smem_u32(&ctl->done), 0, abort_flag, p.status, kStatusDense);
+            if (!ok)
+                for (int i = 0; i < 64; ++i) __nanosleep(2000);   // error path: let copies in flight land
+            __syncwarp();
+        } else if (warp == 10) {
+            // ------------------------------ scales: products s_A s_B of this CTA's 128 rows and both column halves
+            const uint32_t ring = smem_base + kFp8Stages * kFp8StageBytes + kFp8StagingBytes;
+            uint32_t batch = 0, nth = 0;
+            bool ok = true;
+            for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, 1); ok && t.valid(); t.next(), ++nth) {
+                const int row0 = t.m * 256 + static_cast<int>(rank) * 128, col = t.n * 256;
+                // rows and columns past the matrix get scales that exist; what they scale is never stored
+                const float* sa[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sa[r] = p.sfa + (row0 + r * 32 + lane < p.m ? row0 + r * 32 + lane : 0) * p.sfa_row;
+                const float* sb = p.sfb + (col / kFp8Block) * p.sfb_row;
+                const long long next_half = col + 128 < p.n ? p.sfb_row : 0;
+                for (int i0 = 0; i0 < p.k_tiles; i0 += kFp8Batch, ++batch) {
+                    ok = mbar_wait_converged(smem_u32(&ctl->scale_free[batch & 1]), ((batch >> 1) & 1) ^ 1u, abort_flag, p.status, kStatusDense);
+                    if (!ok) break;
+                    if (i0 == 0 && lane == 0) ctl->place[nth & 3] = make_int2(row0, col);
+                    const uint32_t dst = ring + (batch & 1) * kFp8BatchBytes + lane * 4;
+#pragma unroll
+                    for (int part = 0; part < kFp8Batch; part += 4) {
+                        float a[4][4], b[4][2];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int at = i0 + part + j < p.k_tiles ? i0 + part + j : p.k_tiles - 1;
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) a[j][r] = sa[r][at * p.sfa_col];
+                            b[j][0] = sb[at * p.sfb_col];
+                            b[j][1] = sb[at * p.sfb_col + next_half];
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                st_shared_f32(dst + (part + j) * 1024 + r * 128, a[j][r] * b[j][0]);
+                                st_shared_f32(dst + (part + j) * 1024 + 512 + r * 128, a[j][r] * b[j][1]);
+                            }
+                    }
+                    mbar_arrive(smem_u32(&ctl->scale_full[batch & 1]));
+                }
+            }
+            __syncwarp();
+        } else if (warp == 8) {
+            // ------------------------------ MMA issuer
+            if (rank == 0) {
+                constexpr uint32_t kIdesc = idesc_dense(256, 256, 0u, false, false);
+                uint32_t s = 0, ph = 0, cnt = 0;
+                bool ok = true;
+                for (TileWalk t(pair, pairs, p.m_tiles, p.n_tiles, 1); ok && t.valid(); t.next()) {
+#pragma unroll 1
+                    for (int i = 0; i < p.k_tiles; ++i, ++cnt) {
+                        ok = mbar_wait_converged(smem_u32(&ctl->full[s]), ph, abort_flag, p.status, kStatusDense);
+                        if (ok && cnt >= 2)
+                            ok = mbar_wait_converged(smem_u32(&ctl->acc_release[cnt & 1]), ((cnt >> 1) - 1) & 1, abort_flag, p.status,
+                                                     kStatusDense);
+                        if (!ok) break;
+                        tc_fence_after_sync();
+                        const uint32_t a = dense_desc_lo<false>(smem_base + s * kFp8StageBytes);
+                        const uint32_t acc = tmem_base + (cnt & 1) * 256;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)     // 32 e4m3 elements of k = 32 bytes each
+                            tc_mma_f8_pair(acc, a + 2 * j, a + (kFp8OperandBytes >> 4) + 2 * j, kIdesc, j > 0 ? 1u : 0u);
+                        tc_commit_pair_both_elect(smem_u32(&ctl->acc_full[cnt & 1]), 3);
+                        tc_commit_pair_both_elect(smem_u32(&ctl->empty[s]), 3);
+                        if (++s == kFp8Stages) { s = 0; ph ^= 1u; }
+                    }
+                }
+                tc_commit_pair_elect(smem_u32(&ctl->done));
+                mbar_wait<true>(smem_u32(&ctl->done), 0, abort_flag, p.status, kStatusDense);
+            }
+            __syncwarp();
         }
-        __syncwarp();
-      }
     } else {
         warpgroup_reg_inc<kFp8PromoteRegs>();
         // ------------------------------ promotion and epilogue: 32 rows x 128 columns per warp, one row per lane

@@ -347,11 +347,13 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
 }
 
 // The forward pass that also makes the 8-bit copies of g and u.  Tensor memory adds with truncation, one MMA after the other:
-// over a k range of 7168 that left one code in 3400 the neighbour of the right one, 6 to 12 % away, and made the gradients
-// of the weights 1.53 times as far off as their own rounding alone.  So the accumulators are emptied every
-// kKeepChunk steps into fp32 registers (the two accumulators take turns, the MMAs do not wait): one code in XXXX, 1.43 times, and no slower.
+// summed there over k = 7168, one code in 3400 was a neighbour of the right one, 6 to 12 % away, and the weights' gradients were
+// 1.53 times as far off as their own rounding makes them.  So the accumulators are emptied every kKeepChunk steps into fp32
+// registers (the two accumulators take turns, the MMAs do not wait): one code in 27000, 1.43 times, and the same time
+// (m=2048 n=4096 k=7168: 160 us, 156 without the copies).
 // Each of the eight epilogue warps sums 32 rows x 64 columns of g and of u; the two warps of a quadrant agree on a row's largest
-// magnitudes through shared memory.  Registers: 384 threads start with 168; the two epilogue warpgroups take 216, the third keeps 72.
+// magnitudes through shared memory.  Registers: 384 threads start with 168; the two epilogue warpgroups take 216, the third
+// keeps 72 (256 * 216 + 128 * 72 = 384 * 168).
 constexpr int kKeepThreads = 384, kKeepChunk = 16;
 constexpr uint32_t kKeepSumRegs = 216, kKeepOtherRegs = 72;
 static_assert(256 * kKeepSumRegs + 128 * kKeepOtherRegs <= kKeepThreads * 168, "register split");

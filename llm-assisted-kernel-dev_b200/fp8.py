@@ -169,6 +169,8 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_sf: torch.Tensor, *
     A quantised weight is not trained: there is no gradient, and a call that would need one is refused."""
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("fp8_linear has no backward pass: call it under torch.no_grad() or with a detached input")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("fp8_linear: x must be [..., k] with k >= 1")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     _check_activations(x2, "fp8_linear")
     dtype = _dtype_code(x.dtype, "x")

@@ -139,6 +139,9 @@ def gated_ffn(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, *, activation
     keep        what the backward pass works from: "inputs" (x and the weights; the projections are
                 formed again) or "fp8" (8-bit copies of x and of both projections)
 
+    To capture a training step in a CUDA graph, let every eager graph of the same leaves go first and make one call
+    outside the capture (autograd refuses to cross streams inside one, and the library sets itself up on its first call).
+
     fp32 accumulation and gate, one rounding for each of h, dx, dw1, dw2 and for the gradients of the
     two projections, which are operands of the last three.  Runs on the current stream, no synchronisation."""
     _check(x, w1, w2, activation, keep)

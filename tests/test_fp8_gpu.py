@@ -170,12 +170,47 @@ def test_gemm_codes_and_scales_that_make_large_and_small_sums(pkg, dense):
     _check_gemm(dense, pkg.fp8.fp8_gemm(a, sfa, b, sfb), a, sfa, b, sfb)
 
 
-def test_gemm_nan_stays_in_its_row(pkg):
-    x = _rand((50, 384), BF16, 1)
-    x[7, 200] = float("nan")
-    b, sfb = pkg.fp8.quantize_fp8_weight(_rand((136, 384), BF16, 2))
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+@pytest.mark.parametrize("m", [10, 50, 140, 700])
+def test_what_is_not_finite_stays_in_its_row(pkg, m, bad):
+    x = _rand((m, 384), BF16, 1)
+    x[7, 200] = float(bad)
+    b, sfb = pkg.fp8.quantize_fp8_weight(_rand((1032, 384), BF16, 2))
     y = pkg.fp8.fp8_linear(x, b, sfb)
-    assert torch.isnan(y[7]).all() and torch.isfinite(y[[i for i in range(50) if i != 7]]).all()
+    assert torch.isnan(y[7]).all() and torch.isfinite(y[[i for i in range(m) if i != 7]]).all()
+
+
+def test_first_call_under_capture_is_refused():
+    """In a process of its own: the set-up of a device cannot be captured, and says so before it touches the capture."""
+    import subprocess
+    import sys
+    code = """
+import importlib, torch
+pkg = importlib.import_module("llm-assisted-kernel-dev_b200")
+x = torch.ones((4, 128), dtype=torch.bfloat16, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    try:
+        pkg.fp8.quantize_fp8(x)
+        said = None
+    except ValueError as e:
+        said = e.code
+    y = x + 1
+assert said == pkg._lib.E_CAPTURE, said
+g.replay()
+q, sf = pkg.fp8.quantize_fp8(x)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    q, sf = pkg.fp8.quantize_fp8(x)
+g.replay()
+torch.cuda.synchronize()
+assert (y == 2).all() and (pkg.fp8.dequantize_fp8(q, sf).float() - 1).abs().max() < 2 ** -8
+print("fine")
+"""
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
 
 
 @pytest.mark.parametrize("m", [1, 9, 130])
