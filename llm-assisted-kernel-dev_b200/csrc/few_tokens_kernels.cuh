@@ -12,8 +12,8 @@
 //             memory (up to 16 tokens: every tile of W repeats that work, and a launch of its own costs more)
 //   FewGated  16-bit: g and u of the same rows and tokens side by side in tensor memory, h formed after the exchange
 //
-// Warps: four or eight for sums and results, then MMA issuer, weight loads, token loads (and their scales), and four that
-// quantise (kFuse).
+// Warps: four or eight for sums and results, then MMA issuer, weight loads, token loads, and one for scale products (Few8) or four
+// that quantise (kFuse).
 #pragma once
 
 #include "dense_tiles.cuh"
@@ -40,6 +40,8 @@ struct FewProblem {
     uint32_t* status;
 };
 
+constexpr int kFewBatch = 8;             // blocks whose scales are handed over at a time
+
 template <FewOp kOp, int kTokens, bool kFuse> struct FewShape {
     static constexpr bool kFp8 = kOp == FewOp::Few8;
     static constexpr uint32_t kWeightBytes = (kFp8 ? 1u : 2u) * 16384u;     // 128 rows x 128 bytes of each weight
@@ -47,22 +49,26 @@ template <FewOp kOp, int kTokens, bool kFuse> struct FewShape {
     static constexpr uint32_t kStageBytes = kWeightBytes + kTokenBytes;
     // warps that add up the blocks' sums: two for each quadrant of tensor memory with 128 tokens, half of them each
     static constexpr int kSumWarps = kFp8 && kTokens == 128 ? 8 : 4;
-    static constexpr int kThreads = 32 * (kSumWarps + (kFuse ? 7 : 3));
+    static constexpr int kThreads = 32 * (kSumWarps + (kFuse ? 7 : kFp8 ? 4 : 3));
     // two CTAs on an SM up to 64 (fp8) or 32 tokens, one beyond: registers and stages
     static constexpr int kCtasPerSm = kTokens <= (kFp8 ? 64 : 32) ? 2 : 1;
     static constexpr int kStages = static_cast<int>((kCtasPerSm == 2 ? 108u * 1024u : 200u * 1024u) / kStageBytes);
-    static constexpr uint32_t kTmemCols = 2 * kTokens;                      // two block buffers, or g and u
+    static constexpr int kBuffers = kFp8 ? 4 : 1;                           // accumulators that take turns
+    static constexpr uint32_t kTmemCols = (kFp8 ? kBuffers : 2) * kTokens;  // these, or g and u
+    static constexpr int kArrivals = kFuse ? 5 : 2;        // on a stage's barrier: weight loads; token loads or the quantising warps
+    // scales: a slot for each stage (kFuse), or two batches of kFewBatch blocks
+    static constexpr int kScaleRows = kFuse ? kStages : 2 * kFewBatch;
     // partial sums for the exchange take the place of the stages
     static_assert((kFp8 ? 1u : 2u) * kTokens * 512u <= kStages * kStageBytes, "exchange area");
     static_assert(kStageBytes % 1024 == 0, "stages keep the alignment of the swizzle");
 };
 template <FewOp kOp, int kTokens, bool kFuse> struct FewControl {
     using S = FewShape<kOp, kTokens, kFuse>;
-    uint64_t wfull[S::kStages], tfull[S::kStages], empty[S::kStages];
-    uint64_t sfull[S::kStages], sempty[S::kStages];
-    uint64_t acc_full[2], acc_release[2];
+    uint64_t full[S::kStages], empty[S::kStages];
+    uint64_t scale_full[2], scale_free[S::kStages];      // batches; a slot of kFuse is full with its stage
+    uint64_t acc_full[S::kBuffers], acc_release[S::kBuffers];
     uint32_t tmem_base, abort_flag;
-    alignas(16) float scale[S::kStages][kTokens];
+    alignas(16) float scale[S::kScaleRows][kTokens];     // s_A, or s_A s_B
 };
 template <FewOp kOp, int kTokens, bool kFuse> constexpr uint32_t few_smem_bytes() {
     using S = FewShape<kOp, kTokens, kFuse>;
@@ -91,13 +97,58 @@ template <int kN> __device__ __forceinline__ void tc_ld_cols(uint32_t taddr, uin
     else tc_ld_x32(taddr, v);
 }
 
+// Results of the tokens that fall to this warp, from the sums of all ranks.  kGroup tokens of kMost loads each (two of them for
+// the gated block) are in flight before the first is added: one remote load takes about 0.5 us.
+template <FewOp kOp, int kTokens, bool kBf16, int kMost, int kGroup>
+__device__ __forceinline__ void few_sum_ranks(const FewProblem& p, uint32_t area, int w_row, int token0, int tokens, uint32_t rank,
+                                              uint32_t splits, int warp, int warps, int lane) {
+    constexpr bool kFp8 = kOp == FewOp::Few8;
+    const int col = w_row + lane * 4;        // four neighbouring columns of C; n is a multiple of four
+    if (col >= p.n) return;
+    const int step = static_cast<int>(splits) * warps;
+#pragma unroll 1
+    for (int t0 = static_cast<int>(rank + splits * warp); t0 < tokens; t0 += step * kGroup) {
+        float4 g[kGroup][kMost], u[kGroup][kFp8 ? 1 : kMost];
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) {
+            const uint32_t mine = area + (t0 + j * step) * 512 + lane * 16;
+#pragma unroll
+            for (uint32_t r = 0; r < kMost; ++r)
+                if (t0 + j * step < tokens && r < splits) {
+                    g[j][r] = ld_cluster_v4f(map_to_cta(mine, r));
+                    if constexpr (!kFp8) u[j][r] = ld_cluster_v4f(map_to_cta(mine + kTokens * 512, r));
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) {
+            if (t0 + j * step >= tokens) break;
+            float4 y = g[j][0];
+#pragma unroll
+            for (uint32_t r = 1; r < kMost; ++r)
+                if (r < splits) add_v4f(y, g[j][r]);
+            if constexpr (!kFp8) {
+                float4 z = u[j][0];
+#pragma unroll
+                for (uint32_t r = 1; r < kMost; ++r)
+                    if (r < splits) add_v4f(z, u[j][r]);
+                y.x = gate<false>(y.x, p.gelu).value * z.x;
+                y.y = gate<false>(y.y, p.gelu).value * z.y;
+                y.z = gate<false>(y.z, p.gelu).value * z.z;
+                y.w = gate<false>(y.w, p.gelu).value * z.w;
+            }
+            uint16_t* dst = p.c + (token0 + t0 + j * step) * p.ldc + col;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_16<kBf16>(y.x, y.y), pack_16<kBf16>(y.z, y.w));
+        }
+    }
+}
+
 template <FewOp kOp, int kTokens, bool kBf16, bool kFuse = false>
 __global__ void __launch_bounds__(FewShape<kOp, kTokens, kFuse>::kThreads, FewShape<kOp, kTokens, kFuse>::kCtasPerSm)
 few_tokens_gemm(const __grid_constant__ FewProblem p) {
     using S = FewShape<kOp, kTokens, kFuse>;
     constexpr bool kFp8 = S::kFp8;
     constexpr int kStages = S::kStages;
-    constexpr int kSumWarps = S::kSumWarps, kMma = kSumWarps, kLoadW = kSumWarps + 1, kLoadX = kSumWarps + 2;
+    constexpr int kSumWarps = S::kSumWarps, kMma = kSumWarps, kLoadW = kSumWarps + 1, kLoadX = kSumWarps + 2, kScale = kSumWarps + 3;
     constexpr int kMine = kTokens * 4 / kSumWarps;        // tokens of one summing warp
     constexpr int kChunk = kMine < 32 ? kMine : 32;
     constexpr int kFuseAhead = 4;                         // blocks of k whose tokens a quantising half-warp loads at a time
@@ -115,13 +166,12 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
     volatile uint32_t* abort_flag = &ctl->abort_flag;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(smem_u32(&ctl->wfull[s]), 1);
-            mbar_init(smem_u32(&ctl->tfull[s]), kFuse ? 4 : 1);       // kFuse: the quantising warps
+            mbar_init(smem_u32(&ctl->full[s]), S::kArrivals);
             mbar_init(smem_u32(&ctl->empty[s]), 1);
-            mbar_init(smem_u32(&ctl->sfull[s]), 32);
-            mbar_init(smem_u32(&ctl->sempty[s]), kSumWarps);
+            mbar_init(smem_u32(&ctl->scale_free[s]), kSumWarps);
         }
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < 2; ++b) mbar_init(smem_u32(&ctl->scale_full[b]), 32);    // every lane of the scale warp
+        for (int b = 0; b < S::kBuffers; ++b) {
             mbar_init(smem_u32(&ctl->acc_full[b]), 1);
             mbar_init(smem_u32(&ctl->acc_release[b]), kSumWarps);
         }
@@ -162,7 +212,7 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
                 for (int a = 0; a < kFuseAhead; ++a) {
                     if (i0 + a >= count) break;
                     ok = mbar_wait_converged(smem_u32(&ctl->empty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense) &&
-                         mbar_wait_converged(smem_u32(&ctl->sempty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense);
+                         mbar_wait_converged(smem_u32(&ctl->scale_free[s]), ph ^ 1u, abort_flag, p.status, kStatusDense);
                     if (!ok) break;
                     const uint32_t tile = smem_base + s * S::kStageBytes + S::kWeightBytes;
 #pragma unroll
@@ -186,7 +236,7 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
                     }
                     fence_proxy_async_smem();
                     __syncwarp();
-                    mbar_arrive_elect(smem_u32(&ctl->tfull[s]));
+                    mbar_arrive_elect(smem_u32(&ctl->full[s]));
                     if (++s == kStages) { s = 0; ph ^= 1u; }
                 }
             }
@@ -196,47 +246,64 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
         // ------------------------------ loads
         uint32_t s = 0, ph = 0;
         for (int i = 0; i < count; ++i) {
-            ok = mbar_wait<true>(smem_u32(&ctl->empty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense);
-            if (kFp8 && warp == kLoadX && ok)
-                ok = mbar_wait<true>(smem_u32(&ctl->sempty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense);
-            ok = __all_sync(0xffffffffu, ok);
+            ok = mbar_wait_converged(smem_u32(&ctl->empty[s]), ph ^ 1u, abort_flag, p.status, kStatusDense);
             if (!ok) break;
             const uint32_t dst = smem_base + s * S::kStageBytes;
             const int k0 = (begin + i) * (kFp8 ? 128 : 64);
             if (warp == kLoadW) {
-                const uint32_t bar = smem_u32(&ctl->wfull[s]);
+                const uint32_t bar = smem_u32(&ctl->full[s]);
                 mbar_arrive_expect_tx_elect(bar, S::kWeightBytes);
                 tma_load_2d_elect(dst, &p.w[0], bar, k0, w_row);
                 if constexpr (!kFp8) tma_load_2d_elect(dst + 16384, &p.w[1], bar, k0, w_row);
             } else {
-                const uint32_t bar = smem_u32(&ctl->tfull[s]);
+                const uint32_t bar = smem_u32(&ctl->full[s]);
                 mbar_arrive_expect_tx_elect(bar, S::kTokenBytes);
                 tma_load_2d_elect(dst + S::kWeightBytes, &p.x, bar, k0, token0);
-                if constexpr (kFp8) {
-#pragma unroll
-                    for (int t = lane; t < kTokens; t += 32) {
-                        const bool valid = token0 + t < p.m;
-                        const float* src = valid ? p.sfa + (token0 + t) * p.sfa_row + (begin + i) * p.sfa_col : p.sfa;
-                        cp_async_4(smem_u32(&ctl->scale[s][t]), src, valid);
-                    }
-                    cp_async_arrive_noinc(smem_u32(&ctl->sfull[s]));
-                }
             }
             if (++s == kStages) { s = 0; ph ^= 1u; }
         }
-        if (kFp8 && warp == kLoadX) asm volatile("cp.async.wait_all;" ::: "memory");
         if (!ok)
             for (int i = 0; i < 64; ++i) __nanosleep(2000);   // error path: let copies in flight land
+        __syncwarp();
+    } else if (kFp8 && !kFuse && warp == kScale) {
+        // ------------------------------ scales: products s_A s_B, a batch of blocks at a time
+        constexpr int kPer = kTokens / 32 < 1 ? 1 : kTokens / 32;
+        const float* sb = p.sfb + (w_row / kFp8Block) * p.sfb_row + begin * p.sfb_col;
+        const float* sa[kPer];
+#pragma unroll
+        for (int r = 0; r < kPer; ++r) {
+            const int token = token0 + r * 32 + lane;           // tokens past the last get scales that exist; nobody reads their sums
+            sa[r] = p.sfa + (token < p.m ? token : 0) * p.sfa_row + begin * p.sfa_col;
+        }
+        uint32_t batch = 0;
+        for (int i0 = 0; i0 < count; i0 += kFewBatch, ++batch) {
+            ok = mbar_wait_converged(smem_u32(&ctl->scale_free[batch & 1]), ((batch >> 1) & 1) ^ 1u, abort_flag, p.status, kStatusDense);
+            if (!ok) break;
+            float a[kFewBatch][kPer], b[kFewBatch];
+#pragma unroll
+            for (int j = 0; j < kFewBatch; ++j) {
+                const int at = i0 + j < count ? i0 + j : count - 1;
+#pragma unroll
+                for (int r = 0; r < kPer; ++r) a[j][r] = sa[r][at * p.sfa_col];
+                b[j] = sb[at * p.sfb_col];
+            }
+#pragma unroll
+            for (int j = 0; j < kFewBatch; ++j)
+#pragma unroll
+                for (int r = 0; r < kPer; ++r)
+                    if (kTokens >= 32 || lane < kTokens) ctl->scale[(batch & 1) * kFewBatch + j][r * 32 + lane] = a[j][r] * b[j];
+            mbar_arrive(smem_u32(&ctl->scale_full[batch & 1]));
+        }
         __syncwarp();
     } else if (warp == kMma) {
         // ------------------------------ MMA issuer
         constexpr uint32_t kIdesc = idesc_dense(128, kTokens, kFp8 ? 0u : (kBf16 ? 1u : 0u), false, false);
         uint32_t s = 0, ph = 0;
         for (int i = 0; i < count; ++i) {
-            ok = mbar_wait_converged(smem_u32(&ctl->wfull[s]), ph, abort_flag, p.status, kStatusDense) &&
-                 mbar_wait_converged(smem_u32(&ctl->tfull[s]), ph, abort_flag, p.status, kStatusDense);
-            if (kFp8 && ok && i >= 2)
-                ok = mbar_wait_converged(smem_u32(&ctl->acc_release[i & 1]), ((i >> 1) - 1) & 1, abort_flag, p.status, kStatusDense);
+            const int buf = i % S::kBuffers;
+            ok = mbar_wait_converged(smem_u32(&ctl->full[s]), ph, abort_flag, p.status, kStatusDense);
+            if (kFp8 && ok && i >= S::kBuffers)
+                ok = mbar_wait_converged(smem_u32(&ctl->acc_release[buf]), (i / S::kBuffers - 1) & 1, abort_flag, p.status, kStatusDense);
             if (!ok) break;
             tc_fence_after_sync();
             const uint32_t w = dense_desc_lo<false>(smem_base + s * S::kStageBytes);
@@ -244,14 +311,14 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (kFp8) {
-                    tc_mma_f8_one(tmem_base + (i & 1) * kTokens, w + 2 * j, t + 2 * j, kIdesc, j > 0 ? 1u : 0u);
+                    tc_mma_f8_one(tmem_base + buf * kTokens, w + 2 * j, t + 2 * j, kIdesc, j > 0 ? 1u : 0u);
                 } else {
                     const uint32_t more = (i > 0 || j > 0) ? 1u : 0u;
                     tc_mma_f16_one(tmem_base, w + 2 * j, t + 2 * j, kIdesc, more);
                     tc_mma_f16_one(tmem_base + kTokens, w + (16384u >> 4) + 2 * j, t + 2 * j, kIdesc, more);
                 }
             }
-            if constexpr (kFp8) tc_commit_elect(smem_u32(&ctl->acc_full[i & 1]));
+            if constexpr (kFp8) tc_commit_elect(smem_u32(&ctl->acc_full[buf]));
             tc_commit_elect(smem_u32(&ctl->empty[s]));
             if (++s == kStages) { s = 0; ph ^= 1u; }
         }
@@ -263,38 +330,47 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
         uint64_t acc[kMine / 2];
 #pragma unroll
         for (int j = 0; j < kMine / 2; ++j) acc[j] = 0;
-        const bool exists = w_row < p.n;
         const float* sb = p.sfb + (w_row / kFp8Block) * p.sfb_row + begin * p.sfb_col;
-        float b_next = exists && count > 0 ? sb[0] : 0.0f;
+        float b_next = kFuse && count > 0 ? sb[0] : 0.0f;
         const uint32_t lanes = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + (warp >> 2) * kMine;
         uint32_t s = 0, ph = 0;
         for (int i = 0; i < count; ++i) {
             const uint64_t b2 = pack_f32x2(__float_as_uint(b_next), __float_as_uint(b_next));
-            if (i + 1 < count) b_next = sb[(i + 1) * p.sfb_col];
-            // the scales came with the tokens (kFuse) or by copies of their own
-            ok = mbar_wait_converged(smem_u32(kFuse ? &ctl->tfull[s] : &ctl->sfull[s]), ph, abort_flag, p.status, kStatusDense) &&
-                 mbar_wait_converged(smem_u32(&ctl->acc_full[i & 1]), (i >> 1) & 1, abort_flag, p.status, kStatusDense);
+            if (kFuse && i + 1 < count) b_next = sb[(i + 1) * p.sfb_col];
+            // the scales: with their stage, or with their batch; then the sums
+            const int buf = i % S::kBuffers, batch = i / kFewBatch;
+            if constexpr (kFuse)
+                ok = mbar_wait_converged(smem_u32(&ctl->full[s]), ph, abort_flag, p.status, kStatusDense);
+            else if (i % kFewBatch == 0)
+                ok = mbar_wait_converged(smem_u32(&ctl->scale_full[batch & 1]), (batch >> 1) & 1, abort_flag, p.status, kStatusDense);
+            ok = ok && mbar_wait_converged(smem_u32(&ctl->acc_full[buf]), (i / S::kBuffers) & 1, abort_flag, p.status, kStatusDense);
             if (!ok) break;
             tc_fence_after_sync();
-            const uint32_t scales = smem_u32(&ctl->scale[s][(warp >> 2) * kMine]);
+            const int slot = kFuse ? static_cast<int>(s) : (batch & 1) * kFewBatch + i % kFewBatch;
+            const uint32_t scales = smem_u32(&ctl->scale[slot][(warp >> 2) * kMine]);
 #pragma unroll
             for (int c = 0; c < kMine / kChunk; ++c) {
                 uint32_t v[kChunk];
-                tc_ld_cols<kChunk>(lanes + (i & 1) * kTokens + c * kChunk, v);
+                tc_ld_cols<kChunk>(lanes + buf * kTokens + c * kChunk, v);
                 tc_wait_ld();
 #pragma unroll
                 for (int j = 0; j < kChunk / 4; ++j) {
                     uint32_t f0, f1, f2, f3;
                     ld_shared_v4(scales + (c * kChunk + 4 * j) * 4, f0, f1, f2, f3);
-                    fma_f32x2(acc[c * (kChunk / 2) + 2 * j], pack_f32x2(v[4 * j], v[4 * j + 1]), mul_f32x2(pack_f32x2(f0, f1), b2));
-                    fma_f32x2(acc[c * (kChunk / 2) + 2 * j + 1], pack_f32x2(v[4 * j + 2], v[4 * j + 3]),
-                              mul_f32x2(pack_f32x2(f2, f3), b2));
+                    uint64_t lo = pack_f32x2(f0, f1), hi = pack_f32x2(f2, f3);
+                    if constexpr (kFuse) {
+                        lo = mul_f32x2(lo, b2);
+                        hi = mul_f32x2(hi, b2);
+                    }
+                    fma_f32x2(acc[c * (kChunk / 2) + 2 * j], pack_f32x2(v[4 * j], v[4 * j + 1]), lo);
+                    fma_f32x2(acc[c * (kChunk / 2) + 2 * j + 1], pack_f32x2(v[4 * j + 2], v[4 * j + 3]), hi);
                 }
             }
             tc_fence_before_sync();
             __syncwarp();
-            mbar_arrive_elect(smem_u32(&ctl->acc_release[i & 1]));
-            mbar_arrive_elect(smem_u32(&ctl->sempty[s]));
+            mbar_arrive_elect(smem_u32(&ctl->acc_release[buf]));
+            if (kFuse || i % kFewBatch == kFewBatch - 1)
+                mbar_arrive_elect(smem_u32(&ctl->scale_free[kFuse ? static_cast<int>(s) : batch & 1]));
             if (++s == kStages) { s = 0; ph ^= 1u; }
         }
 #pragma unroll
@@ -363,35 +439,12 @@ few_tokens_gemm(const __grid_constant__ FewProblem p) {
         __syncwarp();
         cluster_arrive();
         cluster_wait();
-        // token t is summed by rank t % splits, in rank order; a lane takes four neighbouring columns of C, and all
-        // ranks' loads are in flight before the first is added (one remote load takes about 0.3 us)
-        const int col = w_row + lane * 4;
-        if (warp < kSumWarps && col < p.n) {
-#pragma unroll 2
-            for (int t = rank + splits * warp; t < tokens; t += splits * kSumWarps) {
-                const uint32_t mine = smem_base + t * 512 + lane * 16;
-                float4 g[8], u[kFp8 ? 1 : 8];
-#pragma unroll
-                for (uint32_t r = 0; r < 8; ++r)
-                    if (r < splits) {
-                        g[r] = ld_cluster_v4f(map_to_cta(mine, r));
-                        if constexpr (!kFp8) u[r] = ld_cluster_v4f(map_to_cta(mine + kTokens * 512, r));
-                    }
-#pragma unroll
-                for (uint32_t r = 1; r < 8; ++r)
-                    if (r < splits) {
-                        add_v4f(g[0], g[r]);
-                        if constexpr (!kFp8) add_v4f(u[0], u[r]);
-                    }
-                if constexpr (!kFp8) {
-                    g[0].x = gate<false>(g[0].x, p.gelu).value * u[0].x;
-                    g[0].y = gate<false>(g[0].y, p.gelu).value * u[0].y;
-                    g[0].z = gate<false>(g[0].z, p.gelu).value * u[0].z;
-                    g[0].w = gate<false>(g[0].w, p.gelu).value * u[0].w;
-                }
-                uint16_t* dst = p.c + (token0 + t) * p.ldc + col;       // n, ldc and col are multiples of four
-                *reinterpret_cast<uint2*>(dst) = make_uint2(pack_16<kBf16>(g[0].x, g[0].y), pack_16<kBf16>(g[0].z, g[0].w));
-            }
+        // token t is summed by rank t % splits, in rank order
+        if (warp < kSumWarps) {
+            // tokens at a time: what the registers of one or two CTAs per SM hold
+            constexpr int kFull = (S::kCtasPerSm == 1 ? 2 : 1) * (kFp8 ? 2 : 1);
+            if (splits <= 2) few_sum_ranks<kOp, kTokens, kBf16, 2, 2 * kFull>(p, smem_base, w_row, token0, tokens, rank, splits, warp, kSumWarps, lane);
+            else few_sum_ranks<kOp, kTokens, kBf16, 8, kFull / 2 < 1 ? 1 : kFull / 2>(p, smem_base, w_row, token0, tokens, rank, splits, warp, kSumWarps, lane);
         }
         __syncwarp();
         cluster_arrive();

@@ -295,8 +295,6 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
     using S = FfShape<kN>;
     constexpr int kStages = S::kStages;
     constexpr bool kDual = kMode == FfMode::Forward || kMode == FfMode::GradHidden;
-    constexpr bool kAMn = kMode == FfMode::GradWeight;
-    constexpr bool kBMn = kMode == FfMode::GradWeight || kMode == FfMode::GradInput;
     constexpr int kTileCols = kDual ? kN / 2 : kN;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;

@@ -154,20 +154,6 @@ __device__ __forceinline__ void st_shared_f32(uint32_t addr, float v) {
     asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
-// Asynchronous copies of four bytes into shared memory, completion per thread.
-__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool valid = true) {   // zero when not valid
-    const int bytes = valid ? 4 : 0;
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kPending> __device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
-}
-// Arrival on an mbarrier when this thread's copies so far have landed.
-__device__ __forceinline__ void cp_async_arrive_noinc(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
-}
-
 // TMEM -> registers, 32 consecutive columns of the warp's own lane quadrant.
 __device__ __forceinline__ void tc_ld_x32(uint32_t taddr, uint32_t* v) {
     asm volatile(
