@@ -10,7 +10,13 @@
 // CTA pairs, 256 x 256 tiles.  One 128-wide block of k is 512 clocks of MMA per pair (8192 multiply-adds per
 // clock and SM); meanwhile the eight promotion warps of each SM read the 128 x 256 sums of the block before
 // (tensor memory, two buffers of 256 columns) and add them, scaled, to 128 registers per thread with packed
-// fp32 pairs: 64 fma.f32x2 per thread and block, 128 issue slots per scheduler.
+// fp32 pairs.  That is what bounds the kernel: the 64 fma.f32x2 per thread and block alone take 328 clocks, with the
+// tensor-memory loads and MMAs running beside them 460, and with the hand-overs of the two buffers about 700.
+// Measured for it (clocks per block, this loop without loads): 32 columns at a time 585, 16 warps of 64 columns 623, a
+// test of the next buffer ahead of time 670, one lane polling 850.  In the whole kernel: scales fetched by the promotion
+// warps 1000, tiles found by divisions 600 more per tile, C stored from registers (32 bytes per lane) 1200 more per
+// tile than through boxes.  m=8192 n=14336 k=4096: 414 us in a burst (2.32 PFLOP/s), 470 to 515 under the power cap;
+// the library's product with one scale for each whole matrix 399 there.
 // Twelve warps: 0-7 promotion and epilogue (quadrant w % 4, columns 128 (w / 4) ..), 8 MMA issuer, 9 TMA producer,
 // 10 scale products.
 #pragma once
