@@ -259,7 +259,7 @@ int ff_projections(FfProblem& p, int* tile_n, const void* x, long long ldx, cons
 int quantize_rows_launch(const char* what, const void* x, int dtype, int rows, int k, long long ldx, void* q, long long ldq,
                          float* sf, long long sf_row, long long sf_col, int pow2, DenseCall& call) {
     const long long units = static_cast<long long>(rows) * ((k + kFp8Block - 1) / kFp8Block);
-    constexpr int kPerBlock = kRowThreads / 16 * kRowUnits;
+    constexpr int kPerBlock = kRowThreads / kRowLanes * kRowUnits;
     const long long blocks = (units + kPerBlock - 1) / kPerBlock;
     if (units + kPerBlock > 0xFFFFFFFFll) return fail(B200_E_LIMIT, "%s: %d rows and k=%d are too many blocks", what, rows, k);
     const bool vec = aligned16(x) && ldx % 8 == 0;
@@ -279,7 +279,7 @@ int quantize_rows_launch(const char* what, const void* x, int dtype, int rows, i
 
 int dequantize_rows_launch(const char* what, const void* q, long long ldq, const float* sf, long long sf_row, long long sf_col,
                            int rows, int k, int out_dtype, void* out, long long ldo, DenseCall& call) {
-    const long long blocks = (static_cast<long long>(rows) * ((k + 7) / 8) + 255) / 256;
+    const long long blocks = (static_cast<long long>(rows) * ((k + 15) / 16) + 255) / 256;
     if (blocks * 256 > 0xFFFFFFFFll) return fail(B200_E_LIMIT, "%s: %d rows and k=%d are too many", what, rows, k);
     auto* kernel = out_dtype == B200_DTYPE_BF16 ? &fp8_dequantize_rows<true> : &fp8_dequantize_rows<false>;
     return launch_dense("fp8_dequantize_rows", kernel, dim3(static_cast<unsigned>(blocks)), 256, 0u, call.stream,
@@ -581,7 +581,9 @@ int b200_gated_backward(const void* x, int64_t ldx, const void* kept, size_t kep
     if (kept) {
         const Kept v(const_cast<void*>(kept), m, n, k, keep_x != 0);
         const unsigned row_groups = static_cast<unsigned>((m + kKeptRows - 1) / kKeptRows);
-        const dim3 grid((n + kKeptCols - 1) / kKeptCols, row_groups < 65535u ? row_groups : 65535u);
+        const unsigned column_blocks = (n + kKeptCols - 1) / kKeptCols;
+        const unsigned most = std::max(1u, call.st->sm_count * kKeptBlocksPerSm / column_blocks);
+        const dim3 grid(column_blocks, std::min(std::min(row_groups, most), 65535u));
         auto* kernel = dtype == B200_DTYPE_BF16 ? &gated_grad_kept<true> : &gated_grad_kept<false>;
         if ((rc = launch_dense("gated_grad_kept", kernel, grid, kKeptThreads, 0u, call.stream, (const uint8_t*)v.qg, (const uint8_t*)v.qu,
                                v.ldn, (const float*)v.sg, (const float*)v.su, 1ll, (long long)m, static_cast<const uint16_t*>(dh),

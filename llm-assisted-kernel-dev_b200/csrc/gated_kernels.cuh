@@ -496,13 +496,14 @@ ff_forward_keep(const __grid_constant__ FfProblem p) {
 
 // dg and du from the 8-bit copies of g and u: a streaming pass, 2 bytes of codes, 2 of dh and 4 of results per
 // element.  A thread takes 16 columns of kKeptRows rows, all loaded before the first is used.  Bound by memory: m=2048 n=4096
-// (67 MB) 16.5 us, m=8192 n=14336 (940 MB) 250 us = 3.8 TB/s.
+// (67 MB) 17 us, m=8192 n=14336 (940 MB) 187 us = 5.0 TB/s (250 with one block for each two rows).
 __device__ __forceinline__ uint4 load_codes16(const uint8_t* p, bool all) {
     if (all) return *reinterpret_cast<const uint4*>(p);
     const uint2 v = *reinterpret_cast<const uint2*>(p);
     return make_uint4(v.x, v.y, 0, 0);
 }
 constexpr int kKeptRows = 2, kKeptThreads = 128;
+constexpr unsigned kKeptBlocksPerSm = 14;     // resident twice over: the blocks walk down the rows
 constexpr int kKeptCols = kKeptThreads * 16;
 template <bool kBf16>
 __global__ void __launch_bounds__(kKeptThreads)
