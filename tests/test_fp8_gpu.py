@@ -266,3 +266,67 @@ def test_same_bits_every_time(pkg):
         first = pkg.fp8.fp8_linear(x, b, sfb)
         for _ in range(5):
             assert torch.equal(pkg.fp8.fp8_linear(x, b, sfb), first)
+
+
+def test_offsets_past_32_bits(pkg, dense):
+    """2.2e9 elements: the last rows of codes, scales and product are those of the last rows alone."""
+    m, k, n = 270_000, 8192, 128
+    x = torch.empty((m, k), dtype=BF16, device="cuda")
+    x[:-300] = 1.0
+    x[-300:] = _rand((300, k), BF16, 1)
+    q, sf = pkg.fp8.quantize_fp8(x)
+    q1, sf1 = pkg.fp8.quantize_fp8(x[-300:].clone())
+    assert torch.equal(q[-300:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(sf[-300:], sf1)
+    b, sfb = pkg.fp8.quantize_fp8_weight(_rand((n, k), BF16, 2))
+    y = pkg.fp8.fp8_gemm(q, sf, b, sfb)
+    _check_gemm(dense, y[-300:], q1, sf1, b, sfb)
+    assert torch.equal(y[0].expand(200, n), y[:200]) and torch.equal(y[0], y[-301])
+    back = pkg.fp8.dequantize_fp8(q, sf)
+    assert torch.equal(back[-300:], pkg.fp8.dequantize_fp8(q1, sf1)) and pkg._lib.read_status(0) == 0
+
+
+def test_two_streams_at_once(pkg):
+    b, sfb = pkg.fp8.quantize_fp8_weight(_rand((1032, 2048), BF16, 2))
+    for m in (3, 60, 400):
+        xs = [_rand((m, 2048), BF16, i) for i in range(2)]
+        want = [pkg.fp8.fp8_linear(x, b, sfb) for x in xs]
+        streams = [torch.cuda.Stream() for _ in xs]
+        torch.cuda.synchronize()
+        for _ in range(30):
+            got = []
+            for x, s in zip(xs, streams):
+                with torch.cuda.stream(s):
+                    got.append(pkg.fp8.fp8_linear(x, b, sfb))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, w) for a, w in zip(got, want))
+
+
+def test_refusals(pkg):
+    x = _rand((8, 256), BF16, 1)
+    b, sfb = pkg.fp8.quantize_fp8_weight(_rand((136, 256), BF16, 2))
+    q, sf = pkg.fp8.quantize_fp8(x)
+    bad = [
+        (lambda: pkg.fp8.quantize_fp8(x.float()), "float16 or bfloat16"),
+        (lambda: pkg.fp8.quantize_fp8(x[0]), "matrix"),
+        (lambda: pkg.fp8.quantize_fp8(x.t()), "unit stride"),
+        (lambda: pkg.fp8.quantize_fp8(x[:1].expand(8, 256)), "ldx=0"),
+        (lambda: pkg.fp8.quantize_fp8_weight(x[:0]), "at least one row"),
+        (lambda: pkg.fp8.fp8_gemm(q.float(), sf, b, sfb), "float8_e4m3fn"),
+        (lambda: pkg.fp8.fp8_gemm(q, sf[:4], b, sfb), "scales of a"),
+        (lambda: pkg.fp8.fp8_gemm(q, sf.half(), b, sfb), "float32"),
+        (lambda: pkg.fp8.fp8_gemm(q, sf, b, sfb[:1]), "scales of the weight"),
+        (lambda: pkg.fp8.fp8_gemm(q[:, :128], sf[:, :1], b, sfb), "k=256"),
+        (lambda: pkg.fp8.fp8_gemm(q, sf, b[:132], sfb), "n=132"),
+        (lambda: pkg.fp8.fp8_gemm(q, sf, b, sfb, out_dtype=torch.float32), "out must be"),
+        (lambda: pkg.fp8.fp8_gemm(q, sf, b, sfb, out=torch.empty((8, 128), dtype=BF16, device="cuda")), "out must be"),
+        (lambda: pkg.fp8.fp8_gemm(q, sf, b, sfb, out=torch.empty((8, 140), dtype=BF16, device="cuda")[:, 4:]), "16-byte"),
+        (lambda: pkg.fp8.fp8_linear(x.requires_grad_(), b, sfb), "no backward pass"),
+        (lambda: pkg.fp8.fp8_linear(x.detach()[:, :0], b, sfb), "k >= 1"),
+        (lambda: pkg.fp8.fp8_linear(x.detach(), b, sfb, out=torch.empty((8, 136), dtype=FP16, device="cuda")), "out must be"),
+    ]
+    for call, needle in bad:
+        with pytest.raises(ValueError, match=needle):
+            call()
+    with torch.no_grad():
+        assert pkg.fp8.fp8_linear(x, b, sfb).shape == (8, 136)
+    assert pkg.fp8.fp8_linear(x.detach()[0], b, sfb).shape == (136,)

@@ -314,3 +314,78 @@ def test_block_then_quantised_projection(pkg, dense):
     want, total = av @ bv.t(), av.abs() @ bv.abs().t()
     tol = (4 * 2.0 ** -22 + (s.shape[1] + 2) * 2.0 ** -24) * total
     _within(y, want, tol + _half_step(BF16) * (want.abs() + tol), "y")
+
+
+def test_offsets_past_32_bits(pkg):
+    """2.2e9 hidden elements: the last rows' results are those of the last rows alone, rows of zeros in between."""
+    m, n, k = 130_000, 16896, 64
+    x = torch.zeros((m, k), dtype=BF16, device="cuda")
+    part, w1, w2, dh_part = _inputs(300, n, k, BF16)
+    x[-300:] = part
+    dh = torch.zeros((m, n), dtype=BF16, device="cuda")
+    dh[-300:] = dh_part
+    for keep in ("inputs", "fp8"):
+        small = [t.clone().requires_grad_() for t in (part, w1, w2)]
+        hs = pkg.gated.gated_ffn(*small, keep=keep)
+        want = torch.autograd.grad(hs, small, dh_part)
+        large = [t.detach().requires_grad_() for t in (x, w1, w2)]
+        h = pkg.gated.gated_ffn(*large, keep=keep)
+        assert torch.allclose(h[-300:].float(), hs.float(), rtol=2 ** -7, atol=1e-5) and not h[0].any() and not h[-301].any()
+        dx, dw1, dw2 = torch.autograd.grad(h, large, dh)
+        for got, ref in ((dx[-300:], want[0]), (dw1, want[1]), (dw2, want[2])):
+            assert (got.double() - ref.double()).norm() <= 2 ** -6 * ref.double().norm()
+        assert not dx[0].any() and not dx[-301].any()
+        del h, hs, dx
+    assert pkg._lib.read_status(0) == 0
+
+
+def test_two_streams_at_once(pkg):
+    for m in (5, 100, 400):
+        sets = [[t.requires_grad_() if i < 3 else t for i, t in enumerate(_inputs(m, 264, 520, BF16, seed))] for seed in (1, 2)]
+        want = [torch.autograd.grad(pkg.gated.gated_ffn(*s[:3], keep="fp8"), s[:3], s[3]) for s in sets]
+        streams = [torch.cuda.Stream() for _ in sets]
+        torch.cuda.synchronize()
+        for _ in range(10):
+            got = []
+            for s, st in zip(sets, streams):
+                with torch.cuda.stream(st):
+                    got.append(torch.autograd.grad(pkg.gated.gated_ffn(*s[:3], keep="fp8"), s[:3], s[3]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+def test_shared_and_broadcast_inputs(pkg):
+    """One weight in both places gets the sum of its two gradients; an input seen through zero strides the sum over its rows."""
+    x, w1, w2, dh = _inputs(40, 136, 72, FP16)
+    two = [x.clone().requires_grad_(), w1.clone().requires_grad_(), w1.clone().requires_grad_()]
+    g = torch.autograd.grad(pkg.gated.gated_ffn(*two), two, dh)
+    w = w1.clone().requires_grad_()
+    both, = torch.autograd.grad(pkg.gated.gated_ffn(x, w, w), (w,), dh)
+    assert torch.equal(both, g[1] + g[2])
+    row = x[:1].clone().requires_grad_()
+    spread = x[:1].expand(40, 72).contiguous().requires_grad_()
+    a, = torch.autograd.grad(pkg.gated.gated_ffn(row.expand(40, 72), w1, w2), (row,), dh)
+    b, = torch.autograd.grad(pkg.gated.gated_ffn(spread, w1, w2), (spread,), dh)
+    assert torch.equal(a, b.sum(0, keepdim=True))
+    assert pkg.gated.gated_ffn(x[0], w1, w2).shape == (136,)
+
+
+def test_refusals(pkg):
+    x, w1, w2, _ = _inputs(8, 136, 72, BF16)
+    bad = [
+        (lambda: pkg.gated.gated_ffn(x.float(), w1.float(), w2.float()), "float16 or bfloat16"),
+        (lambda: pkg.gated.gated_ffn(x, w1.half(), w2), "one type"),
+        (lambda: pkg.gated.gated_ffn(x, w1, w2[:128]), "expected x"),
+        (lambda: pkg.gated.gated_ffn(x[:, :64], w1, w2), "expected x"),
+        (lambda: pkg.gated.gated_ffn(x, w1[:132], w2[:132]), "multiples of 8"),
+        (lambda: pkg.gated.gated_ffn(x[:, :68], w1[:, :68], w2[:, :68]), "multiples of 8"),
+        (lambda: pkg.gated.gated_ffn(x, w1.cpu(), w2), "one device"),
+    ]
+    for call, needle in bad:
+        with pytest.raises(ValueError, match=needle):
+            call()
+    leaves = [t.requires_grad_() for t in (x, w1, w2)]
+    h = pkg.gated.gated_ffn(*leaves)
+    g, = torch.autograd.grad(h, (x,), torch.ones_like(h).requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError):            # there is no second derivative
+        torch.autograd.grad(g.sum(), (x,))
