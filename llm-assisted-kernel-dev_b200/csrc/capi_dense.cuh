@@ -79,8 +79,10 @@ struct DenseCall {
         bool& ready = g_dense_ready[device];
         if (!ready && (rc = reject_first_capture())) return;
         if ((rc = device_state(device, &st)) || ready) return;
-        if ((rc = opt_in_smem(fp8_gemm_pair<false>, kFp8SmemBytes))) return;
-        if ((rc = opt_in_smem(fp8_gemm_pair<true>, kFp8SmemBytes))) return;
+        if ((rc = opt_in_smem(fp8_gemm_pair<false, 256>, fp8_smem_bytes<256>()))) return;
+        if ((rc = opt_in_smem(fp8_gemm_pair<true, 256>, fp8_smem_bytes<256>()))) return;
+        if ((rc = opt_in_smem(fp8_gemm_pair<false, 128>, fp8_smem_bytes<128>()))) return;
+        if ((rc = opt_in_smem(fp8_gemm_pair<true, 128>, fp8_smem_bytes<128>()))) return;
         if ((rc = opt_in_few_all<FewOp::Few8>())) return;
         if ((rc = opt_in_few_all<FewOp::FewGated>())) return;
         if ((rc = opt_in_few<FewOp::Few8, 16, true>())) return;
@@ -170,13 +172,15 @@ template <FfMode kMode> int launch_ff(const char* name, FfProblem& p, int tile_n
                         ff_smem_bytes<256>(), call.stream, p);
 }
 
-constexpr long long kFfNarrowCost = 65;   // a 128-wide tile's time in hundredths of a 256-wide one's (62 to 68 measured)
+// A 128-wide tile's time in hundredths of a 256-wide one's (measured: gated 62 to 68, fp8 62 to 68; m=512 n=4096 k=7168 fp8, one
+// round either way: 20.8 us with 128-wide tiles, 26.9 with 256-wide ones).
+constexpr long long kFfNarrowCost = 65, kFp8NarrowCost = 68;
 // Width of the merged B: 128 where whole rounds of 256-wide tiles over the CTA pairs cost more.  `row_tiles` counts every batch.
-int ff_tile_n(int row_tiles, int cols256, int cols128, int sm_count) {
+int pair_tile_n(int row_tiles, int cols256, int cols128, long long narrow_cost, int sm_count) {
     const int pairs = sm_count / 2;
     const long long wide = (static_cast<long long>(row_tiles) * cols256 + pairs - 1) / pairs;
     const long long narrow = (static_cast<long long>(row_tiles) * cols128 + pairs - 1) / pairs;
-    return narrow * kFfNarrowCost < wide * 100 ? 128 : 256;
+    return narrow * narrow_cost < wide * 100 ? 128 : 256;
 }
 
 // CTAs that share the k range of one tile: as many as the GPU has room for, with at least four steps each.
@@ -241,7 +245,7 @@ int ff_projections(FfProblem& p, int* tile_n, const void* x, long long ldx, cons
     int rc;
     p.m_tiles = (m + 255) / 256;
     // 8-bit copies are made from whole 128-wide blocks
-    *tile_n = keep ? 256 : ff_tile_n(p.m_tiles, (n + 127) / 128, (n + 63) / 64, sm_count);
+    *tile_n = keep ? 256 : pair_tile_n(p.m_tiles, (n + 127) / 128, (n + 63) / 64, kFfNarrowCost, sm_count);
     const int cols = *tile_n / 2;
     if ((rc = encode_matrix_map(&p.a[0], x, 2, k, m, ldx, 64, 128))) return rc;
     if ((rc = encode_matrix_map(&p.b[0], w1, 2, k, n, ldw1, 64, cols))) return rc;
@@ -345,7 +349,9 @@ int fp8_gemm_launch(const Fp8Matrix& a, const Fp8Matrix& b, void* c, long long l
     }
     Fp8Problem p;
     if ((rc = encode_matrix_map(&p.a, a.q, 1, k, m, a.ld, 128, 128))) return rc;
-    if ((rc = encode_matrix_map(&p.b, b.q, 1, k, n, b.ld, 128, 128))) return rc;
+    p.m_tiles = (m + 255) / 256;
+    const int tile_n = pair_tile_n(p.m_tiles, (n + 255) / 256, (n + 127) / 128, kFp8NarrowCost, call.st->sm_count);
+    if ((rc = encode_matrix_map(&p.b, b.q, 1, k, n, b.ld, 128, tile_n / 2))) return rc;
     if ((rc = encode_matrix_map(&p.c, c, 2, n, m, ldc, 64, 32))) return rc;
     p.sfa = a.sf;
     p.sfa_row = a.sf_row;
@@ -356,12 +362,15 @@ int fp8_gemm_launch(const Fp8Matrix& a, const Fp8Matrix& b, void* c, long long l
     p.m = m;
     p.n = n;
     p.k_tiles = (k + kFp8Block - 1) / kFp8Block;
-    p.m_tiles = (m + 255) / 256;
-    p.n_tiles = (n + 255) / 256;
+    p.n_tiles = (n + tile_n - 1) / tile_n;
     p.status = status ? status : call.st->status;
     const int grid = pair_grid(static_cast<long long>(p.m_tiles) * p.n_tiles, call.st->sm_count);
-    auto* kernel = out_dtype == B200_DTYPE_BF16 ? &fp8_gemm_pair<true> : &fp8_gemm_pair<false>;
-    return launch_dense("fp8_gemm_pair", kernel, dim3(grid), kFp8Threads, kFp8SmemBytes, call.stream, p);
+    const bool bf16 = out_dtype == B200_DTYPE_BF16;
+    if (tile_n == 128)
+        return launch_dense("fp8_gemm_pair", bf16 ? &fp8_gemm_pair<true, 128> : &fp8_gemm_pair<false, 128>, dim3(grid), kFp8Threads,
+                            fp8_smem_bytes<128>(), call.stream, p);
+    return launch_dense("fp8_gemm_pair", bf16 ? &fp8_gemm_pair<true, 256> : &fp8_gemm_pair<false, 256>, dim3(grid), kFp8Threads,
+                        fp8_smem_bytes<256>(), call.stream, p);
 }
 
 }  // namespace
@@ -619,7 +628,7 @@ int b200_gated_backward(const void* x, int64_t ldx, const void* kept, size_t kep
         p.segments = 2;
         p.m_tiles = (m + 255) / 256;
         p.batches = 1;
-        const int tile_n = ff_tile_n(p.m_tiles, (k + 255) / 256, (k + 127) / 128, call.st->sm_count);
+        const int tile_n = pair_tile_n(p.m_tiles, (k + 255) / 256, (k + 127) / 128, kFfNarrowCost, call.st->sm_count);
         p.n_tiles = (k + tile_n - 1) / tile_n;
         if ((rc = launch_ff<FfMode::GradInput>("ff_gemm_pair<GradInput>", p, tile_n, dtype, call, status))) return rc;
     }
@@ -640,7 +649,7 @@ int b200_gated_backward(const void* x, int64_t ldx, const void* kept, size_t kep
         p.k_tiles = (m + 63) / 64;
         p.segments = 1;
         p.m_tiles = (n + 255) / 256;
-        const int tile_n = ff_tile_n(p.m_tiles * p.batches, (k + 255) / 256, (k + 127) / 128, call.st->sm_count);
+        const int tile_n = pair_tile_n(p.m_tiles * p.batches, (k + 255) / 256, (k + 127) / 128, kFfNarrowCost, call.st->sm_count);
         p.n_tiles = (k + tile_n - 1) / tile_n;
         if ((rc = launch_ff<FfMode::GradWeight>("ff_gemm_pair<GradWeight>", p, tile_n, dtype, call, status))) return rc;
     }
