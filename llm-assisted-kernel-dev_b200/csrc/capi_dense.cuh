@@ -70,8 +70,9 @@ struct DenseCall {
     DeviceGuard guard;
     DeviceState* st = nullptr;
     cudaStream_t stream;
+    int device;
     int rc;
-    DenseCall(int device, void* s) : lock(g_mutex), stream(static_cast<cudaStream_t>(s)) {
+    DenseCall(int device_, void* s) : lock(g_mutex), stream(static_cast<cudaStream_t>(s)), device(device_) {
         if ((rc = guard.enter(device))) return;
         // a thread that has not used CUDA yet (autograd runs backward passes on its own threads) has the device but
         // no context, which the tensor-map encoder asks for: cudaSetDevice makes the device's context current
@@ -183,31 +184,51 @@ int pair_tile_n(int row_tiles, int cols256, int cols128, long long narrow_cost, 
     return narrow * narrow_cost < wide * 100 ? 128 : 256;
 }
 
-// CTAs that share the k range of one tile: as many as the GPU has room for, with at least four steps each.
-int few_splits(long long tiles, int steps, int slots) {
-    int s = 8;
-    while (s > 1 && (tiles * s > slots || steps < 4 * s)) s >>= 1;
-    return s;
+// CTAs that share the k range of one tile: as many as give every tile's cluster a place at the same time, with at least four
+// steps each.  `places[i]`: clusters of 1 << i CTAs that have one.
+int few_splits(long long tiles, int steps, const int (&places)[4]) {
+    int i = 3;
+    while (i > 0 && (tiles > places[i] || steps < (4 << i))) --i;
+    return 1 << i;
 }
 
 template <FewOp kOp, int kTokens, bool kBf16, bool kFuse = false> int launch_few_as(FewProblem& p, DenseCall& call) {
     using S = FewShape<kOp, kTokens, kFuse>;
-    const int tiles = (p.n + 127) / 128, token_tiles = (p.m + kTokens - 1) / kTokens;
-    const int splits = few_splits(static_cast<long long>(tiles) * token_tiles, p.steps, call.st->sm_count * S::kCtasPerSm);
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
-    cfg.gridDim = dim3(tiles * splits, token_tiles, 1);
     cfg.blockDim = dim3(S::kThreads, 1, 1);
     cfg.dynamicSmemBytes = few_smem_bytes<kOp, kTokens, kFuse>();
     cfg.stream = call.stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = splits;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
+    struct Places { int of[4] = {0, 0, 0, 0}; };
+    static std::map<int, Places> known;      // by device; guarded by the call's lock
+    Places& places = known[call.device];
+    if (!places.of[0]) {
+        cfg.numAttrs = 1;
+        // One CTA per SM: what the GPU holds, which for clusters of eight is less than its SMs make up (a GPC's SMs are no multiple
+        // of eight): 16 tiles (n=2048 k=4096, 128 tokens) took 15.2 us in two rounds of eights, 8.7 in one of fours.  Two CTAs per
+        // SM: their number; a cluster or two that start late cost less than halving the loads in flight (32 tiles, n=4096
+        // k=7168: one token 10.6 us with eights, 13.7 with fours).
+        for (int i = 3; i >= 0; --i) {       // the first entry last: it marks the row as complete
+            if (S::kCtasPerSm == 2) {
+                places.of[i] = call.st->sm_count * 2 >> i;
+                continue;
+            }
+            attr[0].val.clusterDim.x = 1 << i;
+            cfg.gridDim = dim3(1 << i, 1, 1);
+            B200_CUDA(cudaOccupancyMaxActiveClusters(&places.of[i], few_tokens_gemm<kOp, kTokens, kBf16, kFuse>, &cfg));
+        }
+    }
+    const int tiles = (p.n + 127) / 128, token_tiles = (p.m + kTokens - 1) / kTokens;
+    const int splits = few_splits(static_cast<long long>(tiles) * token_tiles, p.steps, places.of);
+    cfg.gridDim = dim3(tiles * splits, token_tiles, 1);
+    attr[0].val.clusterDim.x = splits;
     cfg.numAttrs = 2;
     B200_CUDA(cudaLaunchKernelEx(&cfg, few_tokens_gemm<kOp, kTokens, kBf16, kFuse>, p));
     ++g_launches;
@@ -227,15 +248,16 @@ template <FewOp kOp> int launch_few(FewProblem& p, int dtype, DenseCall& call, u
     }
 }
 // Whether the few-token kernel or the CTA-pair kernel is faster.  Up to 64 rows always the former.  Beyond, its tiles are
-// 128 x 128 and it gains as long as two CTAs or more can share the k range of each.  Measured, few-token against pair:
-//   fp8    m=256: n=4096 k=7168 (64 tiles) 19.8 / 26.7 us, n=7168 k=2048 (112) 13.5 / 11.6; m=128 n=14336 k=4096 (112) 21.7 / 18.9
-//   gated  m=256 n=4096 k=7168 (64) 35.4 / 41.1, but with a short k range, where the exchange counts: m=128 n=7168 k=2048 (56)
-//          19.9 / 17.4, m=1024 n=k=1024 (64) 13.3 / 10.5, m=512 n=k=1024 (32) 10.4 / 10.5
-bool few_is_faster(FewOp op, int m, int n, int steps, int sm_count) {
+// 128 x 128; it gains while several CTAs can share the k range of each and k is long enough to pay for the exchange.  Measured,
+// few-token against pair, us:
+//   fp8    n=4096 k=7168: m=128 (32 tiles) 12.9 / 20.1, m=256 (64) 16.4 / 20.2, m=512 (128) 33.6 / 20.9; n=4096 k=2048: m=128
+//          8.0 / 8.4, m=256 8.7 / 8.5; n=2048 k=1024: m=128 6.2 / 5.7, m=512 7.0 / 6.0
+//   gated  n=4096 k=7168: m=128 (32) 26.7 / 31.5, m=256 (64) 33.2 / 32.2; n=2048 k=4096: m=256 (32) 14.2 / 16.8, m=512 (64) 19.6 /
+//          18.3; n=2048 k=1024: m=128 8.6 / 7.3
+bool few_is_faster(FewOp op, int m, int n, int k, int sm_count) {
     if (m <= 64) return true;
     const long long tiles = static_cast<long long>((n + 127) / 128) * ((m + 127) / 128);
-    if (2 * tiles > sm_count) return false;
-    return op == FewOp::Few8 || steps >= 64 || 4 * tiles <= sm_count;
+    return k >= 2048 && (op == FewOp::Few8 ? 2 : 4) * tiles <= sm_count;
 }
 constexpr int kFuseMost = 16;            // rows up to which fp8_linear quantises inside the product's kernel
 
@@ -328,7 +350,7 @@ size_t fp8_codes_bytes(int m, int k) { return static_cast<size_t>(m) * ((k + 15)
 int fp8_gemm_launch(const Fp8Matrix& a, const Fp8Matrix& b, void* c, long long ldc, int out_dtype, int m, int n, int k,
                     bool after_quantiser, DenseCall& call, uint32_t* status) {
     int rc;
-    if (few_is_faster(FewOp::Few8, m, n, (k + kFp8Block - 1) / kFp8Block, call.st->sm_count)) {
+    if (few_is_faster(FewOp::Few8, m, n, k, call.st->sm_count)) {
         FewProblem p;
         memset(&p, 0, sizeof p);
         if ((rc = encode_matrix_map(&p.w[0], b.q, 1, k, n, b.ld, 128, 128))) return rc;
@@ -524,7 +546,7 @@ int b200_gated_forward(const void* x, int64_t ldx, const void* w1, int64_t ldw1,
         return fail(B200_E_WORKSPACE, "%s: the 8-bit copies need %zu bytes, 16-byte aligned", what, b200_gated_kept_bytes(m, n, k, keep_x));
     DenseCall call(device, stream);
     if (call.rc) return call.rc;
-    if (!kept && few_is_faster(FewOp::FewGated, m, n, (k + 63) / 64, call.st->sm_count)) {
+    if (!kept && few_is_faster(FewOp::FewGated, m, n, k, call.st->sm_count)) {
         FewProblem f;
         memset(&f, 0, sizeof f);
         if ((rc = encode_matrix_map(&f.w[0], w1, 2, k, n, ldw1, 64, 128))) return rc;

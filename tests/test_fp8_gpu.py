@@ -130,7 +130,8 @@ def _check_gemm(dense, got, a, sfa, b, sfb):
 GEMM_SIZES = [(1, 8, 1), (1, 128, 128), (1, 4096, 2048), (2, 136, 130), (3, 264, 4000), (16, 512, 512), (17, 1032, 700),
               (31, 128, 7168), (33, 1024, 96), (64, 2048, 1000), (65, 384, 640), (100, 776, 1024), (127, 256, 255),
               (128, 640, 2048), (129, 136, 512), (200, 1000, 333), (256, 256, 128), (257, 264, 136), (300, 520, 2120),
-              (511, 768, 1536), (700, 2056, 520), (1025, 512, 384), (2000, 1288, 264)]
+              (511, 768, 1536), (700, 2056, 520), (1025, 512, 384), (2000, 1288, 264), (1100, 8200, 300), (2300, 2056, 1100),
+              (600, 2600, 1300), (4500, 4104, 130)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])

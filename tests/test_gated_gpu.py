@@ -85,7 +85,7 @@ def _grads_bound(dg, eg, du, eu, x, w1, w2, dtype):
 
 SIZES = [(1, 8, 8), (1, 128, 256), (1, 1000, 2048), (2, 264, 72), (5, 136, 1000), (16, 512, 512), (33, 72, 136), (64, 1032, 264),
          (100, 640, 1032), (128, 128, 64), (129, 136, 200), (256, 256, 128), (257, 392, 520), (300, 1024, 88), (520, 264, 776),
-         (1100, 520, 136)]
+         (1100, 520, 136), (1300, 2600, 200), (600, 1288, 2200)]
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu"])
@@ -151,7 +151,7 @@ def test_kept_copies_and_the_backward_pass_from_them(pkg, dense, m, n, k, dtype,
     assert pkg._lib.read_status(0) == 0
 
 
-@pytest.mark.parametrize("m,n,k", [(5, 16, 24), (130, 72, 264), (300, 520, 200)])
+@pytest.mark.parametrize("m,n,k", [(5, 16, 24), (130, 72, 264), (300, 520, 200), (700, 2600, 2200), (2600, 1288, 520)])
 def test_gradients_are_exact_on_integers(pkg, m, n, k):
     """g is an integer of at least 24 (a column of ones in x, 32 in w1): sigma(g) is 1 in fp32, act(g) = g and act' = 1, so dg = dh u
     and du = dh g are integers below 2^8 and every sum behind dx and dw is exact in fp32: any difference is a mistake."""
