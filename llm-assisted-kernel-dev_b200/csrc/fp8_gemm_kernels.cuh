@@ -38,7 +38,7 @@ struct Fp8Problem {
 constexpr int kFp8Batch = 8;             // blocks whose scales are handed over at a time
 constexpr uint32_t kFp8OperandBytes = 128u * 128u;
 constexpr uint32_t kFp8StagingBytes = 8u * 8192u;            // per promotion warp two boxes of 32 rows x 128 bytes
-constexpr int kFp8Threads = 384;     // warps 10 and 11 only complete the third warpgroup's register hand-back
+constexpr int kFp8Threads = 384;     // warp 11 only completes the third warpgroup's register hand-back
 // Registers: 384 threads start with 168 each; two promotion warpgroups take 216, the third keeps 72 (256 * 216 + 128 * 72 =
 // 384 * 168).
 constexpr uint32_t kFp8PromoteRegs = 216, kFp8OtherRegs = 72;
