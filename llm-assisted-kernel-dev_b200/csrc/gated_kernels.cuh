@@ -350,12 +350,12 @@ ff_gemm_pair(const __grid_constant__ FfProblem p) {
 // The forward pass that also makes the 8-bit copies of g and u.  Tensor memory adds with truncation, one MMA after the other:
 // summed there over k = 7168, one code in 3400 was a neighbour of the right one, 6 to 12 % away, and the weights' gradients were
 // 1.53 times as far off as their own rounding makes them.  So the accumulators are emptied every kKeepChunk steps into fp32
-// registers (the two accumulators take turns, the MMAs do not wait): one code in 27000, 1.43 times, and the same time
-// (m=2048 n=4096 k=7168: 160 us, 156 without the copies).
+// registers (the two accumulators take turns, the MMAs do not wait): one code in 64000, and the same time; with 4 steps one in 93000
+// and 3 % more (m=2048 n=4096 k=7168: 162 us, 158 without the copies; fp32 products on the ordinary pipe: one in 35000).
 // Each of the eight epilogue warps sums 32 rows x 64 columns of g and of u; the two warps of a quadrant agree on a row's largest
 // magnitudes through shared memory.  Registers: 384 threads start with 168; the two epilogue warpgroups take 216, the third
 // keeps 72 (256 * 216 + 128 * 72 = 384 * 168).
-constexpr int kKeepThreads = 384, kKeepChunk = 16;
+constexpr int kKeepThreads = 384, kKeepChunk = 8;
 constexpr uint32_t kKeepSumRegs = 216, kKeepOtherRegs = 72;
 static_assert(256 * kKeepSumRegs + 128 * kKeepOtherRegs <= kKeepThreads * 168, "register split");
 
