@@ -172,25 +172,32 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_sf: torch.Tensor, *
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("fp8_linear: x must be [..., k] with k >= 1")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    _check_activations(x2, "fp8_linear")
-    dtype = _dtype_code(x.dtype, "x")
     m, k = x2.shape
+    dtype, device = _DTYPES.get(x.dtype), x.device
+    # a short call's time is the host's: one expression where everything is as it should be, the checks that say what is not otherwise
+    if not (dtype is not None and x2.is_cuda and x2.stride(1) == 1 and weight.dtype is E4M3 and weight.dim() == 2
+            and weight.shape[1] == k and weight.stride(1) == 1 and weight.device == device and weight_sf.dtype is torch.float32
+            and weight_sf.device == device and weight_sf.shape == (-(-weight.shape[0] // BLOCK), -(-k // BLOCK))):
+        _check_activations(x2, "fp8_linear")
+        dtype = _dtype_code(x.dtype, "x")
+        _check_weight(weight, weight_sf, k, device, "fp8_linear")
     n = weight.shape[0]
-    device = x.device
-    _check_weight(weight, weight_sf, k, device, "fp8_linear")
-    y = torch.empty((m, n), dtype=x.dtype, device=device) if out is None else out if out.dim() == 2 else out.view(-1, out.shape[-1])
-    if out is not None:
+    if out is None:
+        y = x2.new_empty((m, n))
+    else:
+        y = out if out.dim() == 2 else out.view(-1, out.shape[-1])
         _check_out(y, m, n, device, "fp8_linear")
         if out.dtype != x.dtype:
             raise ValueError(f"fp8_linear: out must be {x.dtype}, got {out.dtype}")
     if m:
-        # up to 16 rows are quantised inside the product's kernel
-        nbytes = m * _padded(k, 16) + 4 * m * -(-k // BLOCK) if m > 16 else 0
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        code = _lib.load().b200_fp8_linear(x2.data_ptr(), _row_pitch(x2), dtype, weight.data_ptr(), _row_pitch(weight),
+        # up to 16 rows are quantised inside the product's kernel; scratch in elements of x's two bytes
+        nbytes = m * ((k + 15) // 16 * 16) + 4 * m * -(-k // BLOCK) if m > 16 else 0
+        scratch = x2.new_empty(nbytes // 2) if nbytes else None
+        index = device.index
+        code = _lib.load().b200_fp8_linear(x2.data_ptr(), x2.stride(0) if m > 1 else k, dtype, weight.data_ptr(), _row_pitch(weight),
                                            weight_sf.data_ptr(), weight_sf.stride(0), weight_sf.stride(1), y.data_ptr(),
-                                           _row_pitch(y), m, n, k, scratch.data_ptr() if nbytes else None, nbytes, _raw_stream(device.index),
-                                           device.index, None)
+                                           y.stride(0) if m > 1 else (n + 7) // 8 * 8, m, n, k,
+                                           scratch.data_ptr() if nbytes else None, nbytes, _raw_stream(index), index, None)
         if code:
             _lib.check(code)
     if out is not None:

@@ -72,7 +72,7 @@ def _forward(x, w1, w2, act: int, kept, keep_x: bool):
     m, k = x.shape
     n = w1.shape[0]
     device = x.device
-    h = torch.empty((m, n), dtype=x.dtype, device=device)
+    h = x.new_empty((m, n))
     if m == 0:
         return h
     pitch = fp8._row_pitch
@@ -110,8 +110,9 @@ class _GatedFfn(torch.autograd.Function):
         if m == 0:
             return (dh.new_empty((0, k)) if need_x else None, torch.zeros_like(w1) if need_w1 else None,
                     torch.zeros_like(w2) if need_w2 else None, None, None)
-        make = lambda need, rows: torch.empty((rows, k), dtype=dh.dtype, device=device) if need else None  # noqa: E731
-        dx, dw1, dw2 = make(need_x, m), make(need_w1, n), make(need_w2, n)
+        dx = dh.new_empty((m, k)) if need_x else None
+        dw1 = dh.new_empty((n, k)) if need_w1 else None
+        dw2 = dh.new_empty((n, k)) if need_w2 else None
         address = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         pitch = fp8._row_pitch
         if ctx.keep == "inputs":
@@ -120,7 +121,7 @@ class _GatedFfn(torch.autograd.Function):
         else:
             source = (None, 0, saved.data_ptr(), saved.numel(), saved.numel() != _kept_bytes(m, n, k, False))
             nbytes = 4 * m * n + 2 * m * k
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        scratch = dh.new_empty(nbytes // 2)
         code = _lib.load().b200_gated_backward(*source, w1.data_ptr(), pitch(w1), w2.data_ptr(), pitch(w2), fp8._DTYPES[dh.dtype],
                                                ctx.act, dh.data_ptr(), pitch(dh), address(dx), k, address(dw1), address(dw2), k,
                                                m, n, k, scratch.data_ptr(), nbytes, fp8._raw_stream(device.index),
